@@ -38,6 +38,14 @@ class MoeShape(ctypes.Structure):
 
 _SHAPE_P = ctypes.POINTER(MoeShape)
 
+
+class FfnShape(ctypes.Structure):
+    _fields_ = [("tokens", ctypes.c_int32), ("hidden", ctypes.c_int32), ("intermediate", ctypes.c_int32)]
+
+
+_FFN_P = ctypes.POINTER(FfnShape)
+_I64 = ctypes.c_int64
+
 PROTOTYPES = {
     "cernels_error_string": (ctypes.c_char_p, [ctypes.c_int]),
     "cernels_version": (ctypes.c_int, []),
@@ -65,6 +73,12 @@ PROTOTYPES = {
     "cernels_moe_route": (ctypes.c_int, [_SHAPE_P, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "cernels_moe_gather": (ctypes.c_int, [_VP, _VP, _I32, _I32, _VP, _VP]),
     "cernels_moe_combine": (ctypes.c_int, [_VP, _VP, _VP, _I32, _I32, _I32, _VP, _VP]),
+    "cernels_gated_ffn_workspace_bytes": (ctypes.c_int, [_FFN_P, _I32, ctypes.POINTER(_SZ)]),
+    "cernels_gated_ffn_saved_bytes": (ctypes.c_int, [_FFN_P, ctypes.POINTER(_SZ)]),
+    "cernels_gated_ffn": (ctypes.c_int, [_FFN_P, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
+    "cernels_gated_ffn_forward": (ctypes.c_int, [_FFN_P, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
+    "cernels_gated_ffn_backward": (ctypes.c_int, [_FFN_P, _VP, _I64] + [_VP] * 11 + [_SZ, _VP]),
+    "cernels_ffn_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), _VP]),
     "cernels_workspace_status": (ctypes.c_int, [_SHAPE_P, ctypes.c_int, _VP, ctypes.POINTER(ctypes.c_int), _VP]),
 }
 

@@ -99,6 +99,9 @@ int sm_count_cached() {
 int check_device() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return CERNELS_E_CUDA;
+  // Binds the device's context to this host thread: the driver call that encodes TMA maps needs
+  // one, and a thread whose first CUDA call this is (autograd's) has none yet.
+  if (cudaSetDevice(dev) != cudaSuccess) return CERNELS_E_CUDA;
   int major = 0, minor = 0;
   cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
   cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
@@ -126,6 +129,8 @@ DecodeWorkspace carve_decode_workspace(const cernels_moe_shape& s, void* base) {
 }
 
 int device_sm_count() { return sm_count_cached(); }
+
+int check_sm100() { return check_device(); }
 
 unsigned long long wait_limit_ns(unsigned long long default_ns) {
   const unsigned long long v = g_wait_limit_ns.load(std::memory_order_relaxed);

@@ -164,6 +164,9 @@ cudaError_t launch_router_topk(const void* logits, int bf16, int tokens, int exp
 
 int device_sm_count();
 
+// CERNELS_OK when the current device is one this library is built for.
+int check_sm100();
+
 // Tiled bf16 TMA map with 128-byte swizzle (grouped_gemm.cu).
 bool encode_bf16_map(CUtensorMap* map, const void* ptr, int rank, const uint64_t* dims, const uint64_t* byte_strides,
                      const uint32_t* box);

@@ -1,0 +1,144 @@
+"""The gated feed-forward block outside the routed experts, with its gradient.
+
+``gated_ffn(x, gate_proj, up_proj, down_proj)`` computes ``(silu(x Wg^T) * (x Wu^T)) Wd^T``:
+the dense MLP and the shared expert of the models in :mod:`cernels_b200.registry` (the
+reference runs them as torch modules, src/kops/registry/qwen3_next_moe_experts.py:31-44).
+It is ``torch.ops.cernels_b200.gated_ffn`` too, and differentiable in all four arguments;
+gradients are deterministic. The backward pass keeps, per token, 2F values in 32 bits and F in
+bf16. Like the experts operators it runs on the current stream, takes scratch from torch's
+caching allocator and never synchronises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ops import _check
+
+_BF16 = torch.bfloat16
+
+
+def _rows_ok(x: torch.Tensor) -> bool:
+    return x.stride(1) == 1 and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0))
+
+
+def _validate(x, gate_proj, up_proj, down_proj) -> _lib.FfnShape:
+    _check(x.is_cuda, "x must be a CUDA tensor")
+    _check(x.dim() == 2 and x.dtype == _BF16, "x must be [T, H] bf16")
+    T, H = x.shape
+    for name, w in (("gate_proj", gate_proj), ("up_proj", up_proj), ("down_proj", down_proj)):
+        _check(w.device == x.device, f"{name} must be on {x.device}")
+        _check(w.dim() == 2 and w.dtype == _BF16, f"{name} must be 2-D bf16")
+        _check(w.is_contiguous(), f"{name} must be contiguous")
+    F = gate_proj.shape[0]
+    _check(gate_proj.shape[1] == H and up_proj.shape == gate_proj.shape, "gate_proj and up_proj must be [F, H]")
+    _check(down_proj.shape[0] == H and down_proj.shape[1] == F, "down_proj must be [H, F]")
+    _check(H > 0 and F > 0 and H % 8 == 0 and F % 8 == 0, "H and F must be multiples of 8")
+    _check(_rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least H) apart")
+    return _lib.FfnShape(T, H, F)
+
+
+def _stride(x: torch.Tensor) -> int:
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    """Calls a C-ABI entry, whose last argument is the stream, with `device` current."""
+    fn = getattr(_lib.load(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, name)
+
+
+def _forward(x, gate_proj, up_proj, down_proj) -> torch.Tensor:
+    shape = _validate(x, gate_proj, up_proj, down_proj)
+    out = torch.empty((shape.tokens, shape.hidden), dtype=_BF16, device=x.device)
+    if shape.tokens == 0:
+        return out
+    n = ctypes.c_size_t(0)
+    _lib.check(_lib.load().cernels_gated_ffn_workspace_bytes(ctypes.byref(shape), 0, ctypes.byref(n)), "workspace query")
+    ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+    _call(x.device, "cernels_gated_ffn", ctypes.byref(shape), x.data_ptr(), _stride(x), gate_proj.data_ptr(),
+          up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), ws.data_ptr(), n.value)
+    return out
+
+
+class _GatedFfn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate_proj, up_proj, down_proj):
+        shape = _validate(x, gate_proj, up_proj, down_proj)
+        T, F, dev = shape.tokens, shape.intermediate, x.device
+        out = torch.empty((T, shape.hidden), dtype=_BF16, device=dev)
+        act = torch.empty((T, F), dtype=_BF16, device=dev)
+        n = ctypes.c_size_t(0)
+        _lib.check(_lib.load().cernels_gated_ffn_saved_bytes(ctypes.byref(shape), ctypes.byref(n)), "size query")
+        saved = torch.empty(n.value // 4, dtype=torch.float32, device=dev)
+        if T:
+            _call(dev, "cernels_gated_ffn_forward", ctypes.byref(shape), x.data_ptr(), _stride(x),
+                  gate_proj.data_ptr(), up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), act.data_ptr(),
+                  saved.data_ptr())
+        ctx.save_for_backward(x, gate_proj, up_proj, down_proj, act, saved)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        x, gate_proj, up_proj, down_proj, act, saved = ctx.saved_tensors
+        shape = _lib.FfnShape(x.shape[0], x.shape[1], gate_proj.shape[0])
+        dev = x.device
+        dout = dout.contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
+        grads = [torch.empty(t.shape, dtype=_BF16, device=dev) if need else None
+                 for t, need in zip((x, gate_proj, up_proj, down_proj), ctx.needs_input_grad)]
+        n = ctypes.c_size_t(0)
+        _lib.check(_lib.load().cernels_gated_ffn_workspace_bytes(ctypes.byref(shape), 1, ctypes.byref(n)),
+                   "workspace query")
+        ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        _call(dev, "cernels_gated_ffn_backward", ctypes.byref(shape), x.data_ptr(), _stride(x), gate_proj.data_ptr(),
+              up_proj.data_ptr(), down_proj.data_ptr(), act.data_ptr(), saved.data_ptr(), dout.data_ptr(),
+              *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), n.value)
+        return tuple(grads)
+
+
+def gated_ffn(x: torch.Tensor, gate_proj: torch.Tensor, up_proj: torch.Tensor, down_proj: torch.Tensor) -> torch.Tensor:
+    """``(silu(x @ gate_proj.T) * (x @ up_proj.T)) @ down_proj.T``.
+
+    x [T, H] bf16 whose rows may lie apart (row stride a multiple of 8); gate_proj and up_proj
+    [F, H], down_proj [H, F], contiguous bf16; H and F multiples of 8. Sums run in 32 bits; the
+    product of the halves is rounded to bf16 once, as the second matrix product's operand.
+    """
+    if torch.is_grad_enabled() and (x.requires_grad or gate_proj.requires_grad or up_proj.requires_grad
+                                    or down_proj.requires_grad):
+        return _GatedFfn.apply(x, gate_proj, up_proj, down_proj)
+    return _forward(x, gate_proj, up_proj, down_proj)
+
+
+def _meta(x, gate_proj, up_proj, down_proj):
+    return x.new_empty((x.shape[0], down_proj.shape[0]))
+
+
+def status(device: torch.device | int | None = None) -> int:
+    """0, or the code of a bounded wait that gave up in one of these kernels on `device` since the
+    last call (the results since then are not to be used). Synchronises the current stream."""
+    code = ctypes.c_int(0)
+    dev = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device("cuda", device).index
+                       if isinstance(device, int) else device.index)
+    with torch.cuda.device(dev):
+        _lib.check(_lib.load().cernels_ffn_status(ctypes.byref(code), torch.cuda.current_stream(dev).cuda_stream),
+                   "cernels_ffn_status")
+    return code.value
+
+
+_DEF = torch.library.Library("cernels_b200", "FRAGMENT")
+_DEF.define("gated_ffn(Tensor x, Tensor gate_proj, Tensor up_proj, Tensor down_proj) -> Tensor")
+_DEF.impl("gated_ffn", _forward, "CUDA")
+_DEF.impl("gated_ffn", gated_ffn, "AutogradCUDA")
+_DEF.impl("gated_ffn", _meta, "Meta")

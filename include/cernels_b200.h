@@ -248,6 +248,43 @@ int cernels_ep_status(void* ctx, int* status);
 int cernels_workspace_status(const cernels_moe_shape* shape, int decode, const void* workspace, int* status,
                              void* stream);
 
+/* ---- Gated feed-forward block y = (silu(x Wg^T) * (x Wu^T)) Wd^T, with its backward pass (the
+ * dense and shared-expert layers beside the routed experts; the reference runs them as torch
+ * modules, src/kops/registry/qwen3_next_moe_experts.py:31-44). All bf16, sums in 32 bits:
+ *   x [T, H] with row stride x_stride >= H elements (a multiple of 8), gate_proj / up_proj [F, H],
+ *   down_proj [H, F], out [T, H]; H and F multiples of 8, every pointer 16-byte aligned.
+ * Waits inside the kernels are bounded (cernels_set_wait_limit_ns); one that gives up leaves a
+ * nonzero code in a per-device word that cernels_ffn_status reads. */
+typedef struct cernels_ffn_shape {
+  int32_t tokens;       /* T */
+  int32_t hidden;       /* H */
+  int32_t intermediate; /* F */
+} cernels_ffn_shape;
+
+/* Bytes of scratch of cernels_gated_ffn (backward == 0) or cernels_gated_ffn_backward. */
+int cernels_gated_ffn_workspace_bytes(const cernels_ffn_shape* shape, int32_t backward, size_t* bytes);
+int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_stride, const void* gate_proj,
+                      const void* up_proj, const void* down_proj, void* out, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/* The forward pass of a training step: also fills what the backward pass reads. act [T, F] bf16
+ * is silu(g) * u; saved holds g and u in 32 bits, cernels_gated_ffn_saved_bytes() bytes, in this
+ * library's own order. */
+int cernels_gated_ffn_saved_bytes(const cernels_ffn_shape* shape, size_t* bytes);
+int cernels_gated_ffn_forward(const cernels_ffn_shape* shape, const void* x, int64_t x_stride, const void* gate_proj,
+                              const void* up_proj, const void* down_proj, void* out, void* act, void* saved,
+                              void* stream);
+
+/* Gradients for dout [T, H]; each of dx [T, H], dgate_proj, dup_proj [F, H] and ddown_proj [H, F]
+ * may be NULL (not computed). Deterministic: no atomics. */
+int cernels_gated_ffn_backward(const cernels_ffn_shape* shape, const void* x, int64_t x_stride, const void* gate_proj,
+                               const void* up_proj, const void* down_proj, const void* act, const void* saved,
+                               const void* dout, void* dx, void* dgate_proj, void* dup_proj, void* ddown_proj,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
+/* Reads the current device's status word (0 = ok) and clears it. Synchronises `stream`. */
+int cernels_ffn_status(int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
