@@ -8,6 +8,7 @@ hand-written CUDA kernels in ``cernels_b200/_C/libcernels_b200.so`` (C ABI in
 
 from . import ops  # noqa: F401  (registers torch.ops.cernels_b200.*)
 from .ffn import gated_ffn  # noqa: F401
+from .w4 import linear_w4, moe_experts_decode_w4, quantize_w4  # noqa: F401
 from .ops import (  # noqa: F401
     cohere2_moe_experts,
     cohere2_moe_experts_decode,

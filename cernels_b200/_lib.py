@@ -78,6 +78,10 @@ PROTOTYPES = {
     "cernels_gated_ffn": (ctypes.c_int, [_FFN_P, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _SZ, _VP]),
     "cernels_gated_ffn_forward": (ctypes.c_int, [_FFN_P, _VP, _I64, _VP, _VP, _VP, _VP, _VP, _VP, _VP]),
     "cernels_gated_ffn_backward": (ctypes.c_int, [_FFN_P, _VP, _I64] + [_VP] * 11 + [_SZ, _VP]),
+    "cernels_linear_w4": (ctypes.c_int, [_I32, _I32, _I32, _I32, _VP, _I64, _VP, _VP, _VP, _VP]),
+    "cernels_moe_w4_workspace_bytes": (ctypes.c_int, [_SHAPE_P, _I32, ctypes.POINTER(_SZ)]),
+    "cernels_moe_experts_decode_w4": (ctypes.c_int, [_SHAPE_P, _I32, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _SZ,
+                                                     _VP]),
     "cernels_ffn_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int), _VP]),
     "cernels_workspace_status": (ctypes.c_int, [_SHAPE_P, ctypes.c_int, _VP, ctypes.POINTER(ctypes.c_int), _VP]),
 }

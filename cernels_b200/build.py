@@ -19,7 +19,7 @@ CSRC = PKG_DIR / "csrc"
 OUT_DIR = PKG_DIR / "_C"
 LIB_NAME = "libcernels_b200.so"
 SOURCES = ["capi.cu", "route.cu", "permute.cu", "grouped_gemm.cu", "decode.cu", "capi_noalloc.cu", "router.cu", "router_gemm.cu", "ep_p2p.cu",
-           "pair_gemm.cu", "capi_ffn.cu"]
+           "pair_gemm.cu", "skinny.cu", "capi_ffn.cu"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -41,6 +41,46 @@ size_t act_bytes(const cernels_ffn_shape* s) {
   return align_up(static_cast<size_t>(s->tokens) * s->intermediate * 2, 256);
 }
 
+// A few tokens: the weights' bytes bound the work, and the kernel that streams them reads them at the
+// same rate for 1 to 16 rows.
+bool few(const cernels_ffn_shape* s) { return s->tokens <= kSkinnyMaxColumns; }
+
+int balanced_columns(int tokens, int k) {
+  const int most = skinny_columns(kSkinnyMaxColumns, k);
+  if (most == 0) return 0;
+  const int passes = (tokens + most - 1) / most;
+  return (tokens + passes - 1) / passes;
+}
+
+int check_group(int group, int a, int b) {
+  if (group != 32 && group != 64 && group != 128) return CERNELS_E_UNSUPPORTED;
+  return a % group == 0 && b % group == 0 ? CERNELS_OK : CERNELS_E_INVALID_SHAPE;
+}
+
+int check_moe_w4(const cernels_moe_shape* s, int group) {
+  if (!s) return CERNELS_E_NULL;
+  if (s->tokens < 0 || s->hidden <= 0 || s->experts <= 0 || s->intermediate <= 0 || s->topk <= 0)
+    return CERNELS_E_INVALID_SHAPE;
+  if (s->layout != CERNELS_LAYOUT_LINEAR || s->experts > kMaxExperts) return CERNELS_E_UNSUPPORTED;
+  if (static_cast<long long>(s->tokens) * s->topk > kDecodeMaxPairs) return CERNELS_E_UNSUPPORTED;
+  if (s->hidden > (1 << 16) || s->intermediate > (1 << 16)) return CERNELS_E_UNSUPPORTED;
+  return check_group(group, s->hidden, s->intermediate);
+}
+
+struct MoeW4Workspace {
+  __nv_bfloat16* act;  // [T * topk, F]
+  float* rows;         // [T * topk, H]
+  size_t bytes;
+};
+MoeW4Workspace carve_moe_w4(const cernels_moe_shape* s, void* base) {
+  const size_t pairs = static_cast<size_t>(s->tokens) * s->topk;
+  const size_t act = align_up(pairs * s->intermediate * 2, 256);
+  uint8_t* p = static_cast<uint8_t*>(base);
+  return {reinterpret_cast<__nv_bfloat16*>(p), reinterpret_cast<float*>(p + act), act + pairs * s->hidden * 4};
+}
+
+const uint8_t* bytes(const void* p) { return static_cast<const uint8_t*>(p); }
+const uint16_t* halves(const void* p) { return static_cast<const uint16_t*>(p); }
 const __nv_bfloat16* in(const void* p) { return static_cast<const __nv_bfloat16*>(p); }
 __nv_bfloat16* outp(void* p) { return static_cast<__nv_bfloat16*>(p); }
 
@@ -76,6 +116,32 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
   if (!aligned(out) || !aligned(workspace)) return CERNELS_E_ALIGNMENT;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const FfnShape s = shape_of(shape);
+  if (few(shape) && skinny_columns(1, s.hidden) && skinny_columns(1, s.inter)) {
+    SkinnyArgs a{};
+    a.x = in(x);
+    a.x_stride = static_cast<size_t>(x_stride);
+    a.w0 = bytes(gate_proj);
+    a.w1 = bytes(up_proj);
+    a.out = workspace;
+    a.out_stride = static_cast<size_t>(s.inter);
+    a.k = s.hidden;
+    a.rows = s.inter;
+    a.tokens = s.tokens;
+    a.cols = balanced_columns(s.tokens, s.hidden);
+    cudaError_t e = launch_skinny(a, 0, true, false, st);
+    a.x = in(workspace);
+    a.x_stride = static_cast<size_t>(s.inter);
+    a.w0 = bytes(down_proj);
+    a.w1 = nullptr;
+    a.out = out;
+    a.out_stride = static_cast<size_t>(s.hidden);
+    a.k = s.inter;
+    a.rows = s.hidden;
+    a.cols = balanced_columns(s.tokens, s.inter);
+    a.dependent = 1;
+    if (e == cudaSuccess) e = launch_skinny(a, 0, false, false, st);
+    return code_of(e);
+  }
   cudaError_t err = launch_ffn_gate_up(s, in(x), static_cast<size_t>(x_stride), in(gate_proj), in(up_proj),
                                        outp(workspace), nullptr, st);
   if (err == cudaSuccess) err = launch_ffn_down(s, in(workspace), in(down_proj), outp(out), st);
@@ -131,6 +197,103 @@ int cernels_gated_ffn_backward(const cernels_ffn_shape* shape, const void* x, in
   if (err == cudaSuccess)
     err = launch_ffn_grads(s, in(x), static_cast<size_t>(x_stride), in(gate_proj), in(up_proj), in(act), in(dout),
                            d_gate, d_up, g, st);
+  return code_of(err);
+}
+
+int cernels_linear_w4(int32_t tokens, int32_t out_features, int32_t in_features, int32_t group, const void* x,
+                      int64_t x_stride, const void* qweight, const void* scales, void* out, void* stream) {
+  if (tokens < 0 || out_features <= 0 || in_features <= 0) return CERNELS_E_INVALID_SHAPE;
+  int rc = check_group(group, in_features, in_features);
+  if (rc) return rc;
+  if (in_features > (1 << 16) || out_features > (1 << 24)) return CERNELS_E_UNSUPPORTED;
+  if (tokens == 0) return CERNELS_OK;
+  if (!x || !qweight || !scales || !out) return CERNELS_E_NULL;
+  if (!aligned(x) || !aligned(qweight) || x_stride % 8 != 0) return CERNELS_E_ALIGNMENT;
+  if ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(out)) & 1u) return CERNELS_E_ALIGNMENT;
+  if (x_stride < in_features) return CERNELS_E_INVALID_SHAPE;
+  SkinnyArgs a{};
+  a.x = in(x);
+  a.x_stride = static_cast<size_t>(x_stride);
+  a.w0 = bytes(qweight);
+  a.s0 = halves(scales);
+  a.out = out;
+  a.out_stride = static_cast<size_t>(out_features);
+  a.k = in_features;
+  a.rows = out_features;
+  a.tokens = tokens;
+  a.cols = balanced_columns(tokens, in_features);
+  const long long units = (static_cast<long long>(tokens) / a.cols + 1) * (out_features / 16 + 1);
+  if (units > 0x7fffffffll) return CERNELS_E_UNSUPPORTED;
+  rc = check_sm100();
+  if (rc) return rc;
+  return code_of(launch_skinny(a, group, false, false, static_cast<cudaStream_t>(stream)));
+}
+
+int cernels_moe_w4_workspace_bytes(const cernels_moe_shape* shape, int32_t group, size_t* bytes) {
+  const int rc = check_moe_w4(shape, group);
+  if (rc) return rc;
+  if (!bytes) return CERNELS_E_NULL;
+  *bytes = carve_moe_w4(shape, nullptr).bytes;
+  return CERNELS_OK;
+}
+
+int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group, const void* x, const void* gate_up_q,
+                                  const void* gate_up_scales, const void* down_q, const void* down_scales,
+                                  const int32_t* indices, const float* weights, void* out, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  int rc = check_moe_w4(shape, group);
+  if (rc || shape->tokens == 0) return rc;
+  if (!x || !gate_up_q || !gate_up_scales || !down_q || !down_scales || !indices || !weights || !out)
+    return CERNELS_E_NULL;
+  for (const void* p : {x, gate_up_q, gate_up_scales, down_q, down_scales, const_cast<const void*>(out)})
+    if (!aligned(p)) return CERNELS_E_ALIGNMENT;
+  const MoeW4Workspace ws = carve_moe_w4(shape, workspace);
+  if (!workspace || workspace_bytes < ws.bytes) return CERNELS_E_WORKSPACE;
+  if (!aligned(workspace)) return CERNELS_E_ALIGNMENT;
+  rc = check_sm100();
+  if (rc) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const size_t H = shape->hidden, F = shape->intermediate;
+  SkinnyArgs a{};
+  a.indices = indices;
+  a.pairs = shape->tokens * shape->topk;
+  a.topk = shape->topk;
+  a.experts = shape->experts;
+  a.tokens = shape->tokens;
+  a.x = in(x);
+  a.x_stride = H;
+  a.w0 = bytes(gate_up_q);
+  a.w1 = a.w0 + F * (H / 2);
+  a.w_expert = 2 * F * (H / 2);
+  a.s0 = halves(gate_up_scales);
+  a.s1 = a.s0 + F * (H / group);
+  a.s_expert = 2 * F * (H / group);
+  a.out = ws.act;
+  a.out_stride = F;
+  a.k = shape->hidden;
+  a.rows = shape->intermediate;
+  a.cols = skinny_columns(8, a.k);
+  cudaError_t err = launch_skinny(a, group, true, false, st);
+  if (err != cudaSuccess) return code_of(err);
+  a.x = ws.act;
+  a.x_stride = F;
+  a.x_by_pair = 1;
+  a.w0 = bytes(down_q);
+  a.w1 = nullptr;
+  a.w_expert = H * (F / 2);
+  a.s0 = halves(down_scales);
+  a.s1 = nullptr;
+  a.s_expert = H * (F / group);
+  a.out = ws.rows;
+  a.out_stride = H;
+  a.k = shape->intermediate;
+  a.rows = shape->hidden;
+  a.cols = skinny_columns(8, a.k);
+  a.dependent = 1;
+  err = launch_skinny(a, group, false, true, st);
+  if (err == cudaSuccess)
+    err = launch_weighted_rows(ws.rows, indices, weights, shape->tokens, shape->topk, shape->experts, shape->hidden,
+                               outp(out), st);
   return code_of(err);
 }
 

@@ -40,4 +40,33 @@ inline size_t gate_up_floats(const FfnShape& s) {
   return (static_cast<size_t>(s.tokens) + 31) / 32 * 32 * 2 * static_cast<size_t>(s.inter);
 }
 
+// ---- skinny.cu: a few rows of x times bf16 or 4-bit weights
+constexpr int kSkinnyMaxColumns = 16;
+
+struct SkinnyArgs {
+  const __nv_bfloat16* x;
+  size_t x_stride;            // elements between rows of x
+  const uint8_t *w0, *w1;     // weight rows; gate/up: w0 gate, w1 up
+  size_t w_expert;            // bytes between experts
+  const uint16_t *s0, *s1;    // bf16 group scales of the same rows (4 bits)
+  size_t s_expert;            // scales between experts
+  void* out;                  // bf16 or fp32 [column, rows], out_stride elements apart
+  size_t out_stride;
+  int k, rows;                // reduction length; outputs per column (gate/up: F)
+  int cols;                   // columns that a tile takes at once (skinny_columns())
+  int tokens;                 // columns without routing
+  const int32_t* indices;     // routing: expert of each pair, or null; a pair is a column
+  int pairs, topk, experts;
+  int x_by_pair;              // x rows belong to pairs (else to tokens, pair / topk)
+  int dependent;              // x is written by the kernel launched just before on this stream
+};
+
+// Columns per tile for a reduction of `k`: at most `want`, kSkinnyMaxColumns and what shared memory
+// holds of x. 0 when not even one row fits.
+int skinny_columns(int want, int k);
+// group: 0 for bf16 weights, 32 / 64 / 128 for 4 bits. gate_up: out = silu(w0 x) * (w1 x).
+cudaError_t launch_skinny(const SkinnyArgs& a, int group, bool gate_up, bool out_f32, cudaStream_t stream);
+cudaError_t launch_weighted_rows(const float* rows, const int32_t* indices, const float* weights, int tokens, int topk,
+                                 int experts, int hidden, __nv_bfloat16* out, cudaStream_t stream);
+
 }  // namespace cernels

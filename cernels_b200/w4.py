@@ -1,0 +1,129 @@
+"""Products with 4-bit weights and group scales, for the decode path.
+
+A weight row of K values is stored as K / 2 bytes (two codes a byte, the even position in the low
+half) and K / G bf16 scales, G 32, 64 or 128::
+
+    W[n, k] = (q[n, k] - 8) * scale[n, k // G]
+
+``linear_w4`` is a linear layer for a few rows; ``moe_experts_decode_w4`` is the routed experts'
+decode call (``*_moe_experts_decode``) on such weights, a quarter of the bytes that bound it;
+``quantize_w4`` makes the codes and scales from bf16 weights. The first two are
+``torch.ops.cernels_b200.*`` too. They are for inference: a call that would need a gradient raises.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .ffn import _call, _rows_ok, _stride
+from .ops import DECODE_MAX_PAIRS, _check
+
+_BF16 = torch.bfloat16
+GROUPS = (32, 64, 128)
+
+
+def quantize_w4(weight: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, torch.Tensor]:
+    """(codes [..., K / 2] uint8, scales [..., K / group] bf16) of weight [..., K], each group scaled by
+    its largest magnitude / 7 and rounded to the nearest code (a group of zeros gets scale 0)."""
+    _check(group in GROUPS, f"group must be one of {GROUPS}")
+    _check(weight.dim() >= 2 and weight.is_floating_point(), "weight must be a floating [..., N, K] tensor")
+    _check(weight.shape[-1] % group == 0 and weight.shape[-1] > 0, "K must be a multiple of group")
+    w = weight.detach().float().unflatten(-1, (-1, group))
+    scale = (w.abs().amax(-1) / 7.0).to(_BF16)
+    q = w / torch.where(scale == 0, torch.ones_like(scale), scale).float().unsqueeze(-1)
+    q = (torch.round(q) + 8.0).clamp_(0.0, 15.0).to(torch.uint8).flatten(-2)
+    return q[..., 0::2] | (q[..., 1::2] << 4), scale
+
+
+def _check_no_grad(*tensors: torch.Tensor) -> None:
+    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)),
+           "4-bit products have no gradient: call them under torch.no_grad()")
+
+
+def _check_w4(name: str, q: torch.Tensor, s: torch.Tensor, lead: tuple, k: int, dev: torch.device) -> int:
+    """The group size of codes q [*lead, k / 2] with scales s [*lead, k / G]."""
+    _check(q.device == dev and s.device == dev, f"{name} must be on {dev}")
+    _check(q.dtype == torch.uint8 and s.dtype == _BF16, f"{name}: codes must be uint8 and scales bf16")
+    _check(q.is_contiguous() and s.is_contiguous(), f"{name} must be contiguous")
+    _check(tuple(q.shape) == (*lead, k // 2) and k % 2 == 0, f"{name}: codes must be {[*lead, k // 2]}")
+    _check(tuple(s.shape[:-1]) == lead and s.shape[-1] > 0, f"{name}: scales must be {[*lead, 'K / group']}")
+    group = k // s.shape[-1]
+    _check(group in GROUPS and group * s.shape[-1] == k, f"{name}: group must be one of {GROUPS} and divide K")
+    return group
+
+
+def _linear_w4(x, qweight, scales):
+    _check(x.is_cuda, "x must be a CUDA tensor")
+    _check(x.dim() == 2 and x.dtype == _BF16, "x must be [T, K] bf16")
+    _check(qweight.dim() == 2 and scales.dim() == 2, "qweight must be [N, K / 2] and scales [N, K / group]")
+    T, K = x.shape
+    N = qweight.shape[0]
+    group = _check_w4("qweight", qweight, scales, (N,), K, x.device)
+    _check(_rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least K) apart")
+    out = torch.empty((T, N), dtype=_BF16, device=x.device)
+    if T and N:
+        _call(x.device, "cernels_linear_w4", T, N, K, group, x.data_ptr(), _stride(x), qweight.data_ptr(),
+              scales.data_ptr(), out.data_ptr())
+    return out
+
+
+def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """``x @ W.T`` for 4-bit W: x [T, K] bf16 (rows may lie apart), qweight [N, K / 2] uint8, scales
+    [N, K / G] bf16. Made for up to 16 rows, where the weights' bytes bound it; more rows work, and
+    read the weights once per 16."""
+    _check_no_grad(x, scales)
+    return _linear_w4(x, qweight, scales)
+
+
+def _moe_experts_decode_w4(x, gate_up_q, gate_up_scales, down_q, down_scales, indices, weights, topk):
+    _check(x.is_cuda, "x must be a CUDA tensor")
+    _check(x.dim() == 2 and x.dtype == _BF16 and x.is_contiguous(), "x must be contiguous [T, H] bf16")
+    _check(gate_up_q.dim() == 3 and gate_up_q.shape[1] % 2 == 0, "gate_up_q must be [E, 2F, H / 2]")
+    T, H = x.shape
+    E, F = gate_up_q.shape[0], gate_up_q.shape[1] // 2
+    group = _check_w4("gate_up_q", gate_up_q, gate_up_scales, (E, 2 * F), H, x.device)
+    _check(_check_w4("down_q", down_q, down_scales, (E, H), F, x.device) == group,
+           "gate_up and down weights must have the same group")
+    for name, t, dtype in (("indices", indices, torch.int32), ("weights", weights, torch.float32)):
+        _check(t.device == x.device and t.dtype == dtype and t.is_contiguous() and tuple(t.shape) == (T, topk),
+               f"{name} must be contiguous [T, topk] {dtype} on {x.device}")
+    _check(T * topk <= DECODE_MAX_PAIRS, f"at most {DECODE_MAX_PAIRS} (token, slot) pairs per call")
+    out = torch.empty_like(x)
+    if T == 0:
+        return out
+    shape = _lib.MoeShape(T, H, E, F, topk, _lib.LAYOUT_LINEAR)
+    n = ctypes.c_size_t(0)
+    _lib.check(_lib.load().cernels_moe_w4_workspace_bytes(ctypes.byref(shape), group, ctypes.byref(n)),
+               "workspace query")
+    ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+    _call(x.device, "cernels_moe_experts_decode_w4", ctypes.byref(shape), group, x.data_ptr(), gate_up_q.data_ptr(),
+          gate_up_scales.data_ptr(), down_q.data_ptr(), down_scales.data_ptr(), indices.data_ptr(), weights.data_ptr(),
+          out.data_ptr(), ws.data_ptr(), n.value)
+    return out
+
+
+def moe_experts_decode_w4(x: torch.Tensor, gate_up_q: torch.Tensor, gate_up_scales: torch.Tensor, down_q: torch.Tensor,
+                          down_scales: torch.Tensor, indices: torch.Tensor, weights: torch.Tensor,
+                          topk: int) -> torch.Tensor:
+    """``cohere2_moe_experts_decode`` (and the other experts of its layout) on 4-bit weights.
+
+    x [T, H] bf16; gate_up_q [E, 2F, H / 2], down_q [E, H, F / 2] uint8 with their scales; indices
+    [T, topk] int32 (ids outside [0, E) are skipped), weights [T, topk] fp32. At most 1024 pairs.
+    """
+    _check_no_grad(x, gate_up_scales, down_scales, weights)
+    return _moe_experts_decode_w4(x, gate_up_q, gate_up_scales, down_q, down_scales, indices, weights, topk)
+
+
+_DEF = torch.library.Library("cernels_b200", "FRAGMENT")
+_DEF.define("linear_w4(Tensor x, Tensor qweight, Tensor scales) -> Tensor")
+_DEF.define("moe_experts_decode_w4(Tensor x, Tensor gate_up_q, Tensor gate_up_scales, Tensor down_q, "
+            "Tensor down_scales, Tensor indices, Tensor weights, int topk) -> Tensor")
+_DEF.impl("linear_w4", _linear_w4, "CUDA")
+_DEF.impl("linear_w4", linear_w4, "AutogradCUDA")
+_DEF.impl("linear_w4", lambda x, qweight, scales: x.new_empty((x.shape[0], qweight.shape[0])), "Meta")
+_DEF.impl("moe_experts_decode_w4", _moe_experts_decode_w4, "CUDA")
+_DEF.impl("moe_experts_decode_w4", moe_experts_decode_w4, "AutogradCUDA")
+_DEF.impl("moe_experts_decode_w4", lambda x, *rest: torch.empty_like(x), "Meta")

@@ -282,6 +282,27 @@ int cernels_gated_ffn_backward(const cernels_ffn_shape* shape, const void* x, in
                                const void* dout, void* dx, void* dgate_proj, void* dup_proj, void* ddown_proj,
                                void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- Products with 4-bit weights and group scales, for a few rows (the decode path; no
+ * counterpart in the reference, whose weights are bf16). A weight row of K values is K / 2 bytes,
+ * two codes a byte with the even position in the low half, and K / group bf16 scales:
+ *   W[n, k] = (q[n, k] - 8) * scale[n, k / group],   group 32, 64 or 128, K a multiple of it.
+ * Sums are in 32 bits, weights are never rounded. Pointers 16-byte aligned. */
+
+/* out[t, n] = sum_k x[t, k] W[n, k]: x [T, K] bf16 (row stride x_stride, a multiple of 8), out
+ * [T, N] bf16. Bound by the weights' bytes up to 16 rows; more rows read them once per 16. */
+int cernels_linear_w4(int32_t tokens, int32_t out_features, int32_t in_features, int32_t group, const void* x,
+                      int64_t x_stride, const void* qweight, const void* scales, void* out, void* stream);
+
+/* cernels_moe_experts_decode with 4-bit experts (LINEAR layout): gate_up_q [E, 2F, H / 2], gate_up_scales
+ * [E, 2F, H / group], down_q [E, H, F / 2], down_scales [E, H, F / group]; H and F multiples of group;
+ * T * topk <= 1024. Each touched expert is read once per 8 tokens that chose it; ids outside [0, E) are
+ * skipped (a token with no expert gets zeros); deterministic. */
+int cernels_moe_w4_workspace_bytes(const cernels_moe_shape* shape, int32_t group, size_t* bytes);
+int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group, const void* x, const void* gate_up_q,
+                                  const void* gate_up_scales, const void* down_q, const void* down_scales,
+                                  const int32_t* indices, const float* weights, void* out, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 /* Reads the current device's status word (0 = ok) and clears it. Synchronises `stream`. */
 int cernels_ffn_status(int* status, void* stream);
 

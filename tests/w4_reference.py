@@ -1,0 +1,62 @@
+"""4-bit products in 64 bits, with bounds of their errors (the constants of ffn_reference).
+
+Codes and scales are exact in 64 bits and never rounded by the operator, so a linear layer's error is
+its 32-bit sums' (n * 2^-23 of the sum of magnitudes; one more rounding a group for its scale) and
+the output's rounding. The experts' call adds the rounding of the halved product, as an operand.
+"""
+
+import torch
+
+from tests.ffn_reference import ADD, HALF, SIG, TINY
+
+
+def codes(shape, group, seed, device="cuda"):
+    """Random codes over the whole range and scales of both signs, tiny to large."""
+    gen = torch.Generator(device=device).manual_seed(seed)
+    q = torch.randint(0, 256, (*shape[:-1], shape[-1] // 2), generator=gen, device=device, dtype=torch.uint8)
+    s = torch.randn(*shape[:-1], shape[-1] // group, generator=gen, device=device) * 0.01
+    return q, s.to(torch.bfloat16)
+
+
+def values(q, s):
+    low, high = (q & 15).double() - 8.0, (q >> 4).double() - 8.0
+    v = torch.stack((low, high), -1).flatten(-2)
+    return v * s.double().repeat_interleave(v.shape[-1] // s.shape[-1], -1)
+
+
+def _sum_bound(k, mag):
+    return (k + 2) * ADD * mag
+
+
+def linear(x, q, s):
+    x, w = x.double(), values(q, s)
+    y = x @ w.T
+    e = _sum_bound(x.shape[1], x.abs() @ w.abs().T)
+    return y, e + HALF * (y.abs() + e) + TINY
+
+
+def experts(x, q1, s1, q2, s2, indices, weights):
+    E, F = q1.shape[0], q1.shape[1] // 2
+    x = x.double()
+    y = torch.zeros_like(x)
+    bound = torch.zeros_like(x)
+    mag = torch.zeros_like(x)
+    for t in range(indices.shape[0]):
+        for j in range(indices.shape[1]):
+            e = int(indices[t, j])
+            if not 0 <= e < E:
+                continue
+            w1, w2, p = values(q1[e], s1[e]), values(q2[e], s2[e]), float(weights[t, j])
+            gu, egu = w1 @ x[t], _sum_bound(x.shape[1], w1.abs() @ x[t].abs())
+            g, u, eg, eu = gu[:F], gu[F:], egu[:F], egu[F:]
+            a = g * torch.sigmoid(g)
+            h = a * u
+            eh = u.abs() * (1.1 * eg + SIG * a.abs()) + a.abs() * eu + 1.1 * eg * eu
+            eh = eh + HALF * (h.abs() + eh)
+            r = w2 @ h
+            er = w2.abs() @ eh + _sum_bound(F, w2.abs() @ (h.abs() + eh))
+            y[t] += p * r
+            bound[t] += abs(p) * er
+            mag[t] += abs(p) * (r.abs() + er)
+    bound = bound + (indices.shape[1] + 1) * ADD * mag
+    return y, bound + HALF * (y.abs() + bound) + TINY
