@@ -45,8 +45,8 @@ size_t act_bytes(const cernels_ffn_shape* s) {
 // same rate for 1 to 16 rows.
 bool few(const cernels_ffn_shape* s) { return s->tokens <= kSkinnyMaxColumns; }
 
-int balanced_columns(int tokens, int k) {
-  const int most = skinny_columns(kSkinnyMaxColumns, k);
+int balanced_columns(int tokens, int k, int group) {
+  const int most = skinny_columns(kSkinnyMaxColumns, k, group, 0, 0);
   if (most == 0) return 0;
   const int passes = (tokens + most - 1) / most;
   return (tokens + passes - 1) / passes;
@@ -64,7 +64,10 @@ int check_moe_w4(const cernels_moe_shape* s, int group) {
   if (s->layout != CERNELS_LAYOUT_LINEAR || s->experts > kMaxExperts) return CERNELS_E_UNSUPPORTED;
   if (static_cast<long long>(s->tokens) * s->topk > kDecodeMaxPairs) return CERNELS_E_UNSUPPORTED;
   if (s->hidden > (1 << 16) || s->intermediate > (1 << 16)) return CERNELS_E_UNSUPPORTED;
-  return check_group(group, s->hidden, s->intermediate);
+  const int rc = check_group(group, s->hidden, s->intermediate);
+  if (rc) return rc;
+  const int pairs = s->tokens * s->topk, longest = s->hidden > s->intermediate ? s->hidden : s->intermediate;
+  return skinny_columns(1, longest, group, pairs, s->experts) ? CERNELS_OK : CERNELS_E_UNSUPPORTED;
 }
 
 struct MoeW4Workspace {
@@ -116,7 +119,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
   if (!aligned(out) || !aligned(workspace)) return CERNELS_E_ALIGNMENT;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const FfnShape s = shape_of(shape);
-  if (few(shape) && skinny_columns(1, s.hidden) && skinny_columns(1, s.inter)) {
+  if (few(shape) && skinny_columns(1, s.hidden, 0, 0, 0) && skinny_columns(1, s.inter, 0, 0, 0)) {
     SkinnyArgs a{};
     a.x = in(x);
     a.x_stride = static_cast<size_t>(x_stride);
@@ -127,7 +130,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
     a.k = s.hidden;
     a.rows = s.inter;
     a.tokens = s.tokens;
-    a.cols = balanced_columns(s.tokens, s.hidden);
+    a.cols = balanced_columns(s.tokens, s.hidden, 0);
     cudaError_t e = launch_skinny(a, 0, true, false, st);
     a.x = in(workspace);
     a.x_stride = static_cast<size_t>(s.inter);
@@ -137,7 +140,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
     a.out_stride = static_cast<size_t>(s.hidden);
     a.k = s.inter;
     a.rows = s.hidden;
-    a.cols = balanced_columns(s.tokens, s.inter);
+    a.cols = balanced_columns(s.tokens, s.inter, 0);
     a.dependent = 1;
     if (e == cudaSuccess) e = launch_skinny(a, 0, false, false, st);
     return code_of(e);
@@ -221,7 +224,8 @@ int cernels_linear_w4(int32_t tokens, int32_t out_features, int32_t in_features,
   a.k = in_features;
   a.rows = out_features;
   a.tokens = tokens;
-  a.cols = balanced_columns(tokens, in_features);
+  a.cols = balanced_columns(tokens, in_features, group);
+  if (a.cols == 0) return CERNELS_E_UNSUPPORTED;
   const long long units = (static_cast<long long>(tokens) / a.cols + 1) * (out_features / 16 + 1);
   if (units > 0x7fffffffll) return CERNELS_E_UNSUPPORTED;
   rc = check_sm100();
@@ -272,7 +276,7 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   a.out_stride = F;
   a.k = shape->hidden;
   a.rows = shape->intermediate;
-  a.cols = skinny_columns(8, a.k);
+  a.cols = skinny_columns(8, a.k, group, a.pairs, a.experts);
   cudaError_t err = launch_skinny(a, group, true, false, st);
   if (err != cudaSuccess) return code_of(err);
   a.x = ws.act;
@@ -288,7 +292,7 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   a.out_stride = H;
   a.k = shape->intermediate;
   a.rows = shape->hidden;
-  a.cols = skinny_columns(8, a.k);
+  a.cols = skinny_columns(8, a.k, group, a.pairs, a.experts);
   a.dependent = 1;
   err = launch_skinny(a, group, false, true, st);
   if (err == cudaSuccess)

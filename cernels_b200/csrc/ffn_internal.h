@@ -58,12 +58,13 @@ struct SkinnyArgs {
   const int32_t* indices;     // routing: expert of each pair, or null; a pair is a column
   int pairs, topk, experts;
   int x_by_pair;              // x rows belong to pairs (else to tokens, pair / topk)
+  int k_warps;                // warps that share a tile (the launcher sets it)
   int dependent;              // x is written by the kernel launched just before on this stream
 };
 
-// Columns per tile for a reduction of `k`: at most `want`, kSkinnyMaxColumns and what shared memory
-// holds of x. 0 when not even one row fits.
-int skinny_columns(int want, int k);
+// Columns per tile for a reduction of `k` (group as below; pairs and experts 0 without routing): at
+// most `want`, kSkinnyMaxColumns and what shared memory holds of x. 0 when not even one row fits.
+int skinny_columns(int want, int k, int group, int pairs, int experts);
 // group: 0 for bf16 weights, 32 / 64 / 128 for 4 bits. gate_up: out = silu(w0 x) * (w1 x).
 cudaError_t launch_skinny(const SkinnyArgs& a, int group, bool gate_up, bool out_f32, cudaStream_t stream);
 cudaError_t launch_weighted_rows(const float* rows, const int32_t* indices, const float* weights, int tokens, int topk,

@@ -1,8 +1,10 @@
 """4-bit products in 64 bits, with bounds of their errors (the constants of ffn_reference).
 
 Codes and scales are exact in 64 bits and never rounded by the operator, so a linear layer's error is
-its 32-bit sums' (n * 2^-23 of the sum of magnitudes; one more rounding a group for its scale) and
-the output's rounding. The experts' call adds the rounding of the halved product, as an operand.
+its 32-bit sums' and the output's rounding. The operator sums (128 + q) x within a group of G, from a
+start of -136 sum(x), to get the sum of (q - 8) x: G + 3 roundings of at most 2^-23 of magnitudes that
+add up to (143 + 136) sum|x|; then the K / G groups' sums times their scales, with two roundings each.
+The experts' call adds the rounding of the halved product, as an operand.
 """
 
 import torch
@@ -24,14 +26,18 @@ def values(q, s):
     return v * s.double().repeat_interleave(v.shape[-1] // s.shape[-1], -1)
 
 
-def _sum_bound(k, mag):
-    return (k + 2) * ADD * mag
+def _sum_bound(x, q, s):
+    """Bound of the 32-bit sums of |x| [T, K] with the weights of (q, s) [N, ..]."""
+    groups = s.shape[-1]
+    G = x.shape[1] // groups
+    inside = (G + 3) * ADD * 279 * (x.unflatten(1, (groups, G)).sum(-1) @ s.double().abs().T)
+    return inside + (groups + 2) * ADD * (x @ values(q, s).abs().T + inside)
 
 
 def linear(x, q, s):
     x, w = x.double(), values(q, s)
     y = x @ w.T
-    e = _sum_bound(x.shape[1], x.abs() @ w.abs().T)
+    e = _sum_bound(x.abs(), q, s)
     return y, e + HALF * (y.abs() + e) + TINY
 
 
@@ -47,14 +53,14 @@ def experts(x, q1, s1, q2, s2, indices, weights):
             if not 0 <= e < E:
                 continue
             w1, w2, p = values(q1[e], s1[e]), values(q2[e], s2[e]), float(weights[t, j])
-            gu, egu = w1 @ x[t], _sum_bound(x.shape[1], w1.abs() @ x[t].abs())
+            gu, egu = w1 @ x[t], _sum_bound(x[t:t + 1].abs(), q1[e], s1[e])[0]
             g, u, eg, eu = gu[:F], gu[F:], egu[:F], egu[F:]
             a = g * torch.sigmoid(g)
             h = a * u
             eh = u.abs() * (1.1 * eg + SIG * a.abs()) + a.abs() * eu + 1.1 * eg * eu
             eh = eh + HALF * (h.abs() + eh)
             r = w2 @ h
-            er = w2.abs() @ eh + _sum_bound(F, w2.abs() @ (h.abs() + eh))
+            er = w2.abs() @ eh + _sum_bound((h.abs() + eh)[None], q2[e], s2[e])[0]
             y[t] += p * r
             bound[t] += abs(p) * er
             mag[t] += abs(p) * (r.abs() + er)
