@@ -102,10 +102,16 @@ int check_device() {
   // Binds the device's context to this host thread: the driver call that encodes TMA maps needs
   // one, and a thread whose first CUDA call this is (autograd's) has none yet.
   if (cudaSetDevice(dev) != cudaSuccess) return CERNELS_E_CUDA;
-  int major = 0, minor = 0;
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-  cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
-  if (major != 10 || minor != 0) return CERNELS_E_UNSUPPORTED;  // built for sm_100a only
+  static std::atomic<signed char> known[64];  // 0 not asked yet, 1 sm_100, -1 another device
+  signed char state = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (state == 0) {
+    int major = 0, minor = 0;
+    cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+    cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, dev);
+    state = major == 10 && minor == 0 ? 1 : -1;
+    if (dev < 64) known[dev].store(state, std::memory_order_relaxed);
+  }
+  if (state < 0) return CERNELS_E_UNSUPPORTED;  // built for sm_100a only
   return CERNELS_OK;
 }
 

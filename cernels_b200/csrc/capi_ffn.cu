@@ -46,7 +46,7 @@ size_t act_bytes(const cernels_ffn_shape* s) {
 bool few(const cernels_ffn_shape* s) { return s->tokens <= kSkinnyMaxColumns; }
 
 int balanced_columns(int tokens, int k, int group) {
-  const int most = skinny_columns(kSkinnyMaxColumns, k, group, 0, 0);
+  const int most = skinny_columns(kSkinnyMaxColumns, k, group, 0);
   if (most == 0) return 0;
   const int passes = (tokens + most - 1) / most;
   return (tokens + passes - 1) / passes;
@@ -63,11 +63,11 @@ int check_moe_w4(const cernels_moe_shape* s, int group) {
     return CERNELS_E_INVALID_SHAPE;
   if (s->layout != CERNELS_LAYOUT_LINEAR || s->experts > kMaxExperts) return CERNELS_E_UNSUPPORTED;
   if (static_cast<long long>(s->tokens) * s->topk > kDecodeMaxPairs) return CERNELS_E_UNSUPPORTED;
-  if (s->hidden > (1 << 16) || s->intermediate > (1 << 16)) return CERNELS_E_UNSUPPORTED;
+  if (s->hidden > (1 << 15) || s->intermediate > (1 << 15)) return CERNELS_E_UNSUPPORTED;
   const int rc = check_group(group, s->hidden, s->intermediate);
   if (rc) return rc;
   const int pairs = s->tokens * s->topk, longest = s->hidden > s->intermediate ? s->hidden : s->intermediate;
-  return skinny_columns(1, longest, group, pairs, s->experts) ? CERNELS_OK : CERNELS_E_UNSUPPORTED;
+  return skinny_columns(1, longest, group, pairs) ? CERNELS_OK : CERNELS_E_UNSUPPORTED;
 }
 
 struct MoeW4Workspace {
@@ -119,7 +119,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
   if (!aligned(out) || !aligned(workspace)) return CERNELS_E_ALIGNMENT;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const FfnShape s = shape_of(shape);
-  if (few(shape) && skinny_columns(1, s.hidden, 0, 0, 0) && skinny_columns(1, s.inter, 0, 0, 0)) {
+  if (few(shape) && skinny_columns(1, s.hidden, 0, 0) && skinny_columns(1, s.inter, 0, 0)) {
     SkinnyArgs a{};
     a.x = in(x);
     a.x_stride = static_cast<size_t>(x_stride);
@@ -208,11 +208,12 @@ int cernels_linear_w4(int32_t tokens, int32_t out_features, int32_t in_features,
   if (tokens < 0 || out_features <= 0 || in_features <= 0) return CERNELS_E_INVALID_SHAPE;
   int rc = check_group(group, in_features, in_features);
   if (rc) return rc;
-  if (in_features > (1 << 16) || out_features > (1 << 24)) return CERNELS_E_UNSUPPORTED;
+  if (in_features > (1 << 15) || out_features > (1 << 24)) return CERNELS_E_UNSUPPORTED;
   if (tokens == 0) return CERNELS_OK;
   if (!x || !qweight || !scales || !out) return CERNELS_E_NULL;
   if (!aligned(x) || !aligned(qweight) || x_stride % 8 != 0) return CERNELS_E_ALIGNMENT;
-  if ((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(out)) & 1u) return CERNELS_E_ALIGNMENT;
+  // scales are copied in 4-byte words, outputs written one by one
+  if ((reinterpret_cast<uintptr_t>(scales) & 3u) || (reinterpret_cast<uintptr_t>(out) & 1u)) return CERNELS_E_ALIGNMENT;
   if (x_stride < in_features) return CERNELS_E_INVALID_SHAPE;
   SkinnyArgs a{};
   a.x = in(x);
@@ -276,7 +277,9 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   a.out_stride = F;
   a.k = shape->hidden;
   a.rows = shape->intermediate;
-  a.cols = skinny_columns(8, a.k, group, a.pairs, a.experts);
+  // 4 columns are the cheapest tile; an expert with more pairs is read again for each 4 (or 8)
+  const int want = a.pairs > 4 * a.experts ? 8 : 4;
+  a.cols = skinny_columns(want, a.k, group, a.pairs);
   cudaError_t err = launch_skinny(a, group, true, false, st);
   if (err != cudaSuccess) return code_of(err);
   a.x = ws.act;
@@ -292,7 +295,7 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   a.out_stride = H;
   a.k = shape->intermediate;
   a.rows = shape->hidden;
-  a.cols = skinny_columns(8, a.k, group, a.pairs, a.experts);
+  a.cols = skinny_columns(want, a.k, group, a.pairs);
   a.dependent = 1;
   err = launch_skinny(a, group, false, true, st);
   if (err == cudaSuccess)

@@ -11,40 +11,100 @@
 // weights of the next kDepth steps already on their way into registers, across tile borders:
 // up to 128 KB of weights in flight per SM.
 //
-// mma.sync m16n8k16 does the products: rows of W are the A operand straight from the registers
-// they were loaded into, x columns the B operand. The order of k within the reduction is free as long
-// as A and B agree, so each lane takes 16 contiguous bytes of a row and x is stored to match.
-// tcgen05 would need W in shared memory in its tile layout, a trip that 4-bit weights would make
-// unpacked; the tensor pipe is a small part of the time either way.
+// mma.sync does the products: rows of W are the A operand, x columns the B operand. The order of k
+// within the reduction is free as long as A and B agree, so W is used as it lies in memory and x is
+// stored in shared memory to match. tcgen05 would need W in shared memory in its tile layout, a trip
+// that 4-bit weights would make unpacked; the tensor pipe is a small part of the time either way.
 //
-// 4 bits: two codes at a time become the bf16 pair 128 + q by (word >> 4 i) & 0x000f000f | 0x43004300,
-// exactly. A group's sum starts at -136 sum(x) instead of 0, which turns every 128 + q into q - 8
-// without an instruction per weight; it is exact products added in 32 bits, and the group's scale
-// multiplies it in 32 bits, so weights are never rounded. (Subtracting 136 from each pair instead
-// made the kernel issue-bound: 241 instructions per 16 x 128 weights where HBM's rate leaves 180.)
+// 4 bits: a byte holds two codes, and (byte & 0xf0) ^ 0x80 is 16 (q - 8) as a signed byte: the A operand
+// of the 8-bit mma (m16n8k32), in 3 instructions for 8 codes. (Making bf16 pairs of them took 7 and twice the
+// mma's; that version was bound by instructions at 2.3 TB/s.) So x becomes integers too: in each block of
+// 128, x = 2^e v with |v| < 2^14, e from the block's largest |x|, as v = 256 hi + lo in two signed bytes and
+// two mma's (up to 4 columns: two columns of one mma). This keeps 14 bits below the block's largest value, where
+// bf16 x holds 8 bits of each value: every x within 2^-6 of the largest is exact, the others are rounded by at
+// most 2^-14 of it, far below the rounding of the output. The sums of 16 (q - 8) hi and 16 (q - 8) lo over a
+// group are exact integers of at most 128 * 128 * 128 < 2^22, and they start at the integer whose bits are the float 1.5 * 2^23, so that their own
+// bits are that float plus the sum. From there on it is 32-bit floating arithmetic: scales are never
+// rounded and multiply each group's sum. A block of x that holds an infinity or a NaN makes its row NaN.
 #include "ffn_internal.h"
+
+#include <cmath>
 
 namespace cernels {
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kThreads = 32 * kWarps;
-constexpr int kMaxSmem = 232448;          // per CTA
-constexpr int kTwoCtaSmem = 112 * 1024;   // a CTA within this shares its SM with another
+constexpr int kMaxSmem = 232448;        // per CTA
+constexpr int kSmemPerSm = 228 * 1024;  // 1 KB of it is taken per CTA
+constexpr int kDepth = 3;  // steps in flight per warp
+constexpr int kCtas = 2;   // per SM; fewer where x rows need the shared memory
 
 __device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
 
 __device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Codes i and i + 4 of a word of eight, as the bf16 pair (128 + q_i, 128 + q_{i+4}).
-__device__ __forceinline__ uint32_t codes(uint32_t word, int i) { return ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u; }
-constexpr float kCodeOffset = 136.0f;  // 128 + 8
+// d = c + 16 (q - 8) (rows of W) times bytes of x. c is an operand of its own: the constant start of every
+// group's sums then stays in its registers.
+__device__ __forceinline__ void mma_bytes(int4& d, const int4& c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+      : "=r"(d.x), "=r"(d.y), "=r"(d.z), "=r"(d.w)
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(c.x), "r"(c.y), "r"(c.z), "r"(c.w));
+}
+
+constexpr int kFloatBias = 0x4b400000;       // the bits of 1.5 * 2^23: adding n < 2^22 to them adds n to the float
+constexpr float kFloatBiasValue = 12582912.0f;
+
+// Two 32-bit values at once (FFMA2 and the like: half the instructions of the scalar forms).
+struct Two {
+  unsigned long long v;
+};
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ Two two(int lo, int hi) { return two(__int_as_float(lo), __int_as_float(hi)); }
+__device__ __forceinline__ float2 split(Two a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ Two add(Two a, Two b) {
+  Two r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// Copies `bytes` (4, 8 or 16) to shared memory without a register; reads only the first `valid` of
+// them (0: none) and fills the rest with zeros.
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int valid) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(kBytes), "r"(valid)
+                 : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
 
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
@@ -57,14 +117,14 @@ struct Format {
   static constexpr int kStep = 2 * kHalf;
   static constexpr int kGroups = kFmt == 0 ? 1 : 128 / kFmt;  // per half
   static constexpr int kWords = kFmt == 0 ? 1 : kFmt / 32;    // 8-code words per lane and group
-  static constexpr int kDepth = kFmt == 0 || kFmt == 128 ? 4 : 3;
-};
-
-// One step of one row, as a lane holds it: 16 bytes of each half, and the scales it fetched for its
-// quad (low and high half of a word: consecutive groups).
-struct Piece {
-  uint4 w[2];
-  uint32_t scale;
+  // A warp's ring slot: a step's 16 rows, [half][row][64 bytes], and the words that hold the rows'
+  // 2 kGroups scales, [word][row]; rows may start in the middle of a word. An mma takes the same
+  // group from all lanes, 4 kWords bytes each: rows lie so far apart that those reads meet no bank twice.
+  static constexpr int kRow = kFmt == 64 ? 96 : kFmt == 32 ? 80 : 64;
+  static constexpr int kHalfBytes = 16 * kRow;
+  static constexpr int kScaleWords = kFmt == 0 ? 0 : kGroups + 1;
+  static constexpr int kScaleAt = 2 * kHalfBytes;
+  static constexpr int kSlot = kScaleAt + kScaleWords * 64;
 };
 
 // Bytes in a shared-memory row of x: an odd multiple of 64, so that the 8 lanes of a 16-byte
@@ -77,100 +137,117 @@ struct Item {
   int expert, first, count;  // columns: order[first .. first + count)
 };
 
+// Buffers of the warps' sums: with two, a tile's additions overlap the next tile's products.
+__host__ __device__ constexpr int part_buffers(int warps) { return warps == 8 ? 2 : 1; }
+
 struct SkinnySmem {
-  size_t part, sums, x, count, base, rank, order, items, total;
+  size_t ring, part, units, x, items, ids, lead, rank, first, order, total;
 };
 
-// groups: scale groups in padded_k (0 for bf16)
-__host__ __device__ inline SkinnySmem carve_smem(int cols, int padded_k, int groups, int pairs, int experts) {
+// blocks: of 128 values in padded_k (0 for bf16); pairs: 0 without routing
+__host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int cols, int padded_k, int blocks, int pairs) {
   SkinnySmem s;
   size_t off = 0;
+  s.ring = off;
+  off += static_cast<size_t>(warps) * kDepth * slot;
   s.part = off;
-  off += static_cast<size_t>(2) * kWarps * ((cols + 7) / 8 * 8) * 16 * 4;
-  s.sums = off;  // [group][column]: -136 times the group's sum of x
-  off += static_cast<size_t>(groups) * ((cols + 7) / 8 * 8) * 4;
+  off += static_cast<size_t>(part_buffers(warps)) * warps * (cols > 8 ? 16 : cols > 4 ? 8 : 4) * 16 * 4;
+  s.units = off;  // per column and block: 2^e / 16
+  off += (static_cast<size_t>(blocks) * cols * 4 + 15) / 16 * 16;
   s.x = off;
   off += static_cast<size_t>(cols) * x_row_bytes(padded_k);
-  s.count = off;  // the lists exist only with routing
-  off += static_cast<size_t>(experts) * 4;
-  s.base = off;
-  off += static_cast<size_t>(experts) * 4;
+  const size_t n = (static_cast<size_t>(pairs) + 3) / 4 * 4;
+  s.ids = off;
+  off += n * 4;
   s.items = off;
-  off += static_cast<size_t>(pairs) * sizeof(Item);
+  off += n * sizeof(Item);
+  s.lead = off;
+  off += n * 4;
   s.rank = off;
-  off += static_cast<size_t>(pairs) * 2;
+  off += n * 2;
+  s.first = off;
+  off += n * 2;
   s.order = off;
-  off += static_cast<size_t>(pairs) * 2;
+  off += n * 2;
   s.total = off + 16;
   return s;
 }
 
 // Groups the (token, slot) pairs by expert, experts in order of first use and pairs in their own
-// order, into items of at most `cols` columns. Every CTA does this for itself. Returns the items.
+// order, into items of at most `cols` columns. Every CTA does this for itself, each pair by
+// comparing itself with all others (one warp walking through them took 4 us for 232 pairs). Returns the
+// number of items.
 __device__ int build_items(const SkinnyArgs& a, uint8_t* smem, const SkinnySmem& lay) {
-  int* count = reinterpret_cast<int*>(smem + lay.count);
-  int* base = reinterpret_cast<int*>(smem + lay.base);
-  uint16_t* rank = reinterpret_cast<uint16_t*>(smem + lay.rank);
-  uint16_t* order = reinterpret_cast<uint16_t*>(smem + lay.order);
+  int* ids = reinterpret_cast<int*>(smem + lay.ids);
   Item* items = reinterpret_cast<Item*>(smem + lay.items);
+  uint32_t* lead = reinterpret_cast<uint32_t*>(smem + lay.lead);  // an expert's first pair: items << 16 | pairs before it
+  uint16_t* rank = reinterpret_cast<uint16_t*>(smem + lay.rank);
+  uint16_t* first = reinterpret_cast<uint16_t*>(smem + lay.first);
+  uint16_t* order = reinterpret_cast<uint16_t*>(smem + lay.order);
   int* n_items = reinterpret_cast<int*>(smem + lay.total - 16);
-  for (int i = threadIdx.x; i < a.experts; i += kThreads) count[i] = 0;
+  const int padded = (a.pairs + 3) / 4 * 4;
+  for (int p = threadIdx.x; p < padded; p += blockDim.x) {
+    const int e = p < a.pairs ? a.indices[p] : -1;
+    ids[p] = e >= 0 && e < a.experts ? e : -1;
+  }
   __syncthreads();
-  const int lane = threadIdx.x & 31;
-  if (threadIdx.x < 32) {
-    for (int p0 = 0; p0 < a.pairs; p0 += 32) {
-      const int p = p0 + lane;
-      const int e = p < a.pairs ? a.indices[p] : -1;
-      const bool live = e >= 0 && e < a.experts;
-      const unsigned same = __match_any_sync(0xffffffffu, live ? e : -1);
-      const int before = live ? count[e] : 0;
-      const int mine = __popc(same & ((1u << lane) - 1u));
-      if (live) rank[p] = static_cast<uint16_t>(before + mine);
-      __syncwarp();
-      if (live && mine == 0) count[e] = before + __popc(same);
-      __syncwarp();
+  for (int p = threadIdx.x; p < a.pairs; p += blockDim.x) {
+    const int e = ids[p];
+    int before = 0, all = 0, at = p;
+    for (int i = 0; i < padded; i += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(ids + i);
+      const int other[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool same = other[j] == e;
+        all += same;
+        before += same && i + j < p;
+        if (same) at = min(at, i + j);
+      }
     }
-    int pos = 0, item = 0;
+    rank[p] = static_cast<uint16_t>(before);
+    first[p] = static_cast<uint16_t>(at);
+    lead[p] = e >= 0 && before == 0 ? static_cast<uint32_t>((all + a.cols - 1) / a.cols) << 16 | all : 0;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int lane = threadIdx.x;
+    uint32_t total = 0;
     for (int p0 = 0; p0 < a.pairs; p0 += 32) {
       const int p = p0 + lane;
-      const int e = p < a.pairs ? a.indices[p] : -1;
-      const bool first = e >= 0 && e < a.experts && rank[p] == 0;
-      const int n = first ? count[e] : 0;
-      const int parts = (n + a.cols - 1) / a.cols;
-      int pos_incl = n, item_incl = parts;
+      const uint32_t mine = p < a.pairs ? lead[p] : 0;
+      uint32_t sum = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, pos_incl, d), w = __shfl_up_sync(0xffffffffu, item_incl, d);
-        if (lane >= d) {
-          pos_incl += v;
-          item_incl += w;
-        }
+        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += v;
       }
-      if (first) {
-        const int at = pos + pos_incl - n, it = item + item_incl - parts;
-        base[e] = at;
-        for (int i = 0; i < parts; ++i) items[it + i] = Item{e, at + i * a.cols, min(a.cols, n - i * a.cols)};
+      const uint32_t start = total + sum - mine;
+      if (mine != 0) {
+        lead[p] = start;
+        const int n = mine & 0xffff, from = start & 0xffff;
+        Item* to = items + (start >> 16);
+        for (int i = 0; i * a.cols < n; ++i) to[i] = Item{ids[p], from + i * a.cols, min(a.cols, n - i * a.cols)};
       }
-      pos += __shfl_sync(0xffffffffu, pos_incl, 31);
-      item += __shfl_sync(0xffffffffu, item_incl, 31);
+      total += __shfl_sync(0xffffffffu, sum, 31);
     }
-    if (lane == 0) *n_items = item;
+    if (lane == 0) *n_items = total >> 16;
   }
   __syncthreads();
-  for (int p = threadIdx.x; p < a.pairs; p += kThreads) {
-    const int e = a.indices[p];
-    if (e >= 0 && e < a.experts) order[base[e] + rank[p]] = static_cast<uint16_t>(p);
-  }
-  const int n = *n_items;
+  for (int p = threadIdx.x; p < a.pairs; p += blockDim.x)
+    if (ids[p] >= 0) order[(lead[first[p]] & 0xffff) + rank[p]] = static_cast<uint16_t>(p);
   __syncthreads();
-  return n;
+  return *n_items;
 }
 
-template <int kFmt, bool kGateUp, int NT, bool kOutF32>
-__global__ void __launch_bounds__(kThreads, 2) skinny_kernel(const SkinnyArgs a) {
+template <int kFmt, bool kGateUp, int kCols, bool kOutF32, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_kernel(const SkinnyArgs a) {
   using F = Format<kFmt>;
-  constexpr int kDepth = F::kDepth;
-  constexpr int kCols = NT * 8;
+  constexpr int kThreads = 32 * kWarps;
+  // Up to 4 columns of 4-bit products fit one mma: its columns are hi and lo of each.
+  constexpr bool kPacked = kCols == 4;
+  constexpr int NT = kPacked ? 1 : kCols / 8;
+  static_assert(!kPacked || kFmt != 0, "bf16 x has no halves");
   constexpr int kOut = kGateUp ? 8 : 16;  // outputs per tile and column
   extern __shared__ __align__(16) uint8_t smem[];
   let_next_kernel_start();
@@ -183,10 +260,11 @@ __global__ void __launch_bounds__(kThreads, 2) skinny_kernel(const SkinnyArgs a)
   const int padded_k = steps * F::kStep;
   const int x_bytes = x_row_bytes(padded_k);
   const bool routed = a.indices != nullptr;
-  const SkinnySmem lay = carve_smem(a.cols, padded_k, kFmt == 0 ? 0 : padded_k / (kFmt == 0 ? 1 : kFmt),
-                                    routed ? a.pairs : 0, routed ? a.experts : 0);
+  const SkinnySmem lay = carve_smem(kWarps, F::kSlot, a.cols, padded_k, kFmt == 0 ? 0 : padded_k / 128,
+                                    routed ? a.pairs : 0);
   float* part = reinterpret_cast<float*>(smem + lay.part);
-  float* sums = reinterpret_cast<float*>(smem + lay.sums);
+  const int blocks = padded_k / 128;
+  float* units_of_x = reinterpret_cast<float*>(smem + lay.units);  // [column][block]
   uint8_t* xs = smem + lay.x;
   const Item* items = reinterpret_cast<const Item*>(smem + lay.items);
   const uint16_t* order = reinterpret_cast<const uint16_t*>(smem + lay.order);
@@ -208,131 +286,151 @@ __global__ void __launch_bounds__(kThreads, 2) skinny_kernel(const SkinnyArgs a)
   // ---- weights: this lane's two rows of a unit, and the stream of steps through them
   const size_t row_bytes = kFmt == 0 ? static_cast<size_t>(a.k) * 2 : static_cast<size_t>(a.k) / 2;
   const int row_groups = kFmt == 0 ? 0 : a.k / (kFmt == 0 ? 1 : kFmt);
+  constexpr int kPerStep = kFmt == 0 ? 64 : 2 * F::kGroups;  // values (bf16) or groups
   int load_item = begin / per_item, load_unit = begin - load_item * per_item;  // position of the stream
   int load_left = (end - begin) * per_warp, load_step = kw;
   const uint8_t *wa = nullptr, *wb = nullptr;
-  const uint16_t *sa = nullptr, *sb = nullptr;
+  const uint16_t* sw = nullptr;  // scales of the row that this lane fetches them for, from a word's start
+  int s_odd = 0;                 // that row's scales start at the word's second half
+  uint32_t odd_a = 0, odd_b = 0;  // the same for the rows it computes, of the unit being consumed
   auto point = [&] {
     const int e = routed ? items[load_item].expert : 0;
-    const int first = (load_unit * tiles_at_once + rt) * kOut + g;
-    const int ra = min(first, a.rows - 1);
-    const int rb = kGateUp ? ra : min(first + 8, a.rows - 1);
+    const int base = (load_unit * tiles_at_once + rt) * kOut;
+    const int ra = min(base + g, a.rows - 1);
+    const int rb = kGateUp ? ra : min(base + g + 8, a.rows - 1);
     const uint8_t* second = kGateUp ? a.w1 : a.w0;
-    wa = a.w0 + static_cast<size_t>(e) * a.w_expert + static_cast<size_t>(ra) * row_bytes + q * (kFmt == 0 ? 16 : kFmt / 8);
-    wb = second + static_cast<size_t>(e) * a.w_expert + static_cast<size_t>(rb) * row_bytes + q * (kFmt == 0 ? 16 : kFmt / 8);
+    const int at = kw * 128 + q * 16;
+    wa = a.w0 + static_cast<size_t>(e) * a.w_expert + static_cast<size_t>(ra) * row_bytes + at;
+    wb = second + static_cast<size_t>(e) * a.w_expert + static_cast<size_t>(rb) * row_bytes + at;
     if constexpr (kFmt != 0) {
-      const uint16_t* s_second = kGateUp ? a.s1 : a.s0;
-      sa = a.s0 + static_cast<size_t>(e) * a.s_expert + static_cast<size_t>(ra) * row_groups;
-      sb = s_second + static_cast<size_t>(e) * a.s_expert + static_cast<size_t>(rb) * row_groups;
+      const int r = lane & 15;
+      const int row = min(base + (kGateUp ? r & 7 : r), a.rows - 1);
+      const uint16_t* from = (kGateUp && r >= 8 ? a.s1 : a.s0) + static_cast<size_t>(e) * a.s_expert +
+                             static_cast<size_t>(row) * row_groups + kw * kPerStep;
+      s_odd = static_cast<int>(reinterpret_cast<uintptr_t>(from) >> 1 & 1);
+      sw = from - s_odd;
     }
   };
-  // Lane q holds the 16 (128-code groups), 8 (64) or 4 bytes (32) of its quarter of every group, so
-  // that an mma never spans two groups.
-  auto fetch = [&](const uint8_t* w, const uint16_t* s, int step) {
-    Piece p;
-    const uint8_t* src = w + static_cast<size_t>(step) * 128;
-    p.scale = 0;
+  // Lane q copies bytes 16 q of its two rows' halves. `left`: groups (bf16: values) of the row from
+  // this step on.
+  uint8_t* ring = smem + lay.ring + static_cast<size_t>(warp) * kDepth * F::kSlot;
+  const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+  auto copy_half = [&](uint32_t dst, const uint8_t* w, int h, bool whole, int left) {
+    const int first = kFmt == 0 ? h * 32 + q * 8 : h * F::kGroups + q * F::kGroups / 4;
+    copy_async<16>(dst, w + h * 64, whole || first < left ? 16 : 0);
+  };
+  int load_slot = 0;
+  auto issue = [&] {
+    if (load_left != 0) {
+      const int left = (kFmt == 0 ? a.k : row_groups) - load_step * kPerStep;
+      const uint32_t at = ring_at + load_slot * F::kSlot;
+      const uint32_t dst = at + g * F::kRow + q * 16;
+      const bool whole = left >= kPerStep;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      p.w[h] = make_uint4(0, 0, 0, 0);
-      if constexpr (kFmt == 0) {
-        if (step * 64 + h * 32 + q * 8 < a.k) p.w[h] = __ldcs(reinterpret_cast<const uint4*>(src + h * 64));
-      } else {
-        const int left = row_groups - (2 * step + h) * F::kGroups;  // groups from this half on
-        if constexpr (kFmt == 128) {
-          if (left > 0) p.w[h] = __ldcs(reinterpret_cast<const uint4*>(src + h * 64));
-        } else if constexpr (kFmt == 64) {
-          uint2 v[2] = {make_uint2(0, 0), make_uint2(0, 0)};
+      for (int h = 0; h < 2; ++h) {
+        copy_half(dst + h * F::kHalfBytes, wa, h, whole, left);
+        copy_half(dst + h * F::kHalfBytes + 8 * F::kRow, wb, h, whole, left);
+      }
+      wa += a.k_warps * 128;
+      wb += a.k_warps * 128;
+      if constexpr (kFmt != 0) {
+        // two words of 16 rows at a time: this lane's row (lane % 16) and words lane / 16, + 2, ..
+        const uint32_t to = at + F::kScaleAt + lane * 4;
+        const int need = left > 0 ? min(left, 2 * F::kGroups) + s_odd : 0;  // scales from the word's start on
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            if (i < left) v[i] = __ldcs(reinterpret_cast<const uint2*>(src + h * 64 + 32 * i));
-          p.w[h] = make_uint4(v[0].x, v[0].y, v[1].x, v[1].y);
-        } else {
-          uint32_t v[4] = {0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (i < left) v[i] = __ldcs(reinterpret_cast<const uint32_t*>(src + h * 64 + 16 * i));
-          p.w[h] = make_uint4(v[0], v[1], v[2], v[3]);
+        for (int i = 0; i < (F::kScaleWords + 1) / 2; ++i) {
+          const int word = 2 * i + (lane >> 4);
+          if (word < F::kScaleWords) copy_async<4>(to + i * 128, sw + 2 * word, max(0, min(4, 2 * (need - 2 * word))));
         }
+        sw += a.k_warps * kPerStep;
+      }
+      load_slot = load_slot + 1 == kDepth ? 0 : load_slot + 1;
+      --load_left;
+      load_step += a.k_warps;
+      if (load_step - kw == per_warp * a.k_warps) {
+        load_step = kw;
+        if (++load_unit == per_item) {
+          load_unit = 0;
+          ++load_item;
+        }
+        if (load_left != 0) point();
       }
     }
-    if constexpr (kFmt != 0) {
-      // a step has 2, 4 or 8 groups per row: lane q of the quad fetches one, or two neighbours
-      const int first = step * 2 * F::kGroups;
-      if constexpr (kFmt == 32) {
-        const int at = first + 2 * q;
-        if (at < row_groups) p.scale = __ldg(s + at);
-        if (at + 1 < row_groups) p.scale |= static_cast<uint32_t>(__ldg(s + at + 1)) << 16;
-      } else {
-        const int at = first + (q % (2 * F::kGroups));
-        if (at < row_groups) p.scale = __ldg(s + at);
-      }
-    }
-    return p;
+    commit_copies();
   };
-  // scale of group i of the step (0 .. 2 kGroups - 1) from the lane of the quad that fetched it
-  auto scale_of = [&](const Piece& p, int i) {
-    if constexpr (kFmt == 32) {
-      const uint32_t v = __shfl_sync(0xffffffffu, p.scale, (lane & ~3) | (i >> 1));
-      return __uint_as_float(i & 1 ? v & 0xffff0000u : v << 16);
-    } else {
-      return __uint_as_float(__shfl_sync(0xffffffffu, p.scale, (lane & ~3) | i) << 16);
-    }
-  };
-
-  Piece pa[kDepth], pb[kDepth];
   point();
-  auto issue = [&](int d) {
-    if (load_left == 0) return;
-    pa[d] = fetch(wa, sa, load_step);
-    pb[d] = fetch(wb, sb, load_step);
-    --load_left;
-    load_step += a.k_warps;
-    if (load_step - kw == per_warp * a.k_warps) {
-      load_step = kw;
-      if (++load_unit == per_item) {
-        load_unit = 0;
-        ++load_item;
-      }
-      if (load_left != 0) point();
-    }
-  };
 #pragma unroll
-  for (int d = 0; d < kDepth; ++d) issue(d);
-
+  for (int d = 0; d < kDepth; ++d) issue();
   if (a.dependent) wait_for_previous_kernel();  // x is the previous kernel's output
 
-  // ---- x rows of an item, 8 values at a time, in the order in which the weights lie in the lanes
+  // ---- x rows of an item, 8 values (a piece) at a time, in the order in which the weights lie
   auto load_x = [&](const Item& it) {
-    const int pieces = padded_k / 8;  // a multiple of 32 with 4-bit weights: a warp stays within a row
-    for (int i = threadIdx.x; i < it.count * pieces; i += kThreads) {
-      const int c = i / pieces, k8 = i - c * pieces;
-      int row = it.first + c;
-      if (routed) {
-        row = order[row];
-        if (!a.x_by_pair) row /= a.topk;
+    const unsigned pieces = static_cast<unsigned>(padded_k) / 8;  // 4 bits: a multiple of 32, so a warp stays within a row
+    const unsigned total = it.count * pieces;
+    if constexpr (kFmt == 0) {
+      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(xs));
+      for (unsigned i = threadIdx.x; i < total; i += kThreads) {
+        const unsigned c = i / pieces, k8 = i - c * pieces;
+        const size_t row = it.first + c;
+        copy_async<16>(to + c * x_bytes + k8 * 16, a.x + row * a.x_stride + k8 * 8, static_cast<int>(k8) * 8 < a.k ? 16 : 0);
       }
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (k8 * 8 < a.k) v = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(row) * a.x_stride + k8 * 8);
-      int at = k8;
-      if constexpr (kFmt != 0) {
-        constexpr int kPer = kFmt / 8;  // pieces (lanes here) per group
-        float sum = 0.f;
+      commit_copies();
+      wait_copies<0>();
+      return;
+    }
+    constexpr int kBatch = 8;  // loads on their way at once
+    for (unsigned i0 = threadIdx.x; i0 < total; i0 += kThreads * kBatch) {
+      uint4 v[kBatch];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint32_t u = j == 0 ? v.x : j == 1 ? v.y : j == 2 ? v.z : v.w;
-          sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xffff0000u);
+      for (int b = 0; b < kBatch; ++b) {
+        const unsigned i = i0 + b * kThreads;
+        v[b] = make_uint4(0, 0, 0, 0);
+        if (i < total) {
+          const unsigned c = i / pieces, k8 = i - c * pieces;
+          int row = it.first + static_cast<int>(c);
+          if (routed) {
+            row = order[row];
+            if (!a.x_by_pair) row /= a.topk;
+          }
+          if (static_cast<int>(k8) * 8 < a.k)
+            v[b] = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(row) * a.x_stride + k8 * 8);
         }
-#pragma unroll
-        for (int d = kPer / 2; d > 0; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        const int in = k8 % kPer;
-        if (in == 0) sums[(k8 / kPer) * kCols + c] = -kCodeOffset * sum;
-        // group | quarter | word  ->  group | word | quarter, and pairs (i, i + 4)
-        at = k8 - in + (in % F::kWords) * 4 + in / F::kWords;
-        v = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410),
-                       __byte_perm(v.y, v.w, 0x7632));
       }
-      *reinterpret_cast<uint4*>(xs + static_cast<size_t>(c) * x_bytes + at * 16) = v;
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const unsigned i = i0 + b * kThreads;
+        if (i >= total) break;  // whole warps, where lanes work together
+        const unsigned c = i / pieces, k8 = i - c * pieces;
+        unsigned at = k8;
+        if constexpr (kFmt != 0) {
+          const uint32_t words[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+          uint32_t top = 0;  // largest magnitude, as bits
+#pragma unroll
+          for (int j = 0; j < 4; ++j) top = max(top, max(words[j] << 16 & 0x7fff0000u, words[j] & 0x7fff0000u));
+#pragma unroll
+          for (unsigned d = 8; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+          // 2^13 <= largest / 2^e < 2^14 (less for values whose unit, or its 16th, would be subnormal)
+          const int unit_exp = max(static_cast<int>(top >> 23) - 13, 5);
+          const float inverse = __uint_as_float(static_cast<uint32_t>(254 - unit_exp) << 23);
+          uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};  // even and odd positions
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const uint32_t bits = j & 1 ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16;
+            // the nearest integer in the low half of the float's bits, in two's complement
+            const uint32_t n = __float_as_uint(fmaf(__uint_as_float(bits), inverse, kFloatBiasValue));
+            hi[j & 1] |= (n + 128 >> 8 & 255u) << (8 * (j >> 1));
+            lo[j & 1] |= (n & 255u) << (8 * (j >> 1));
+          }
+          if (k8 % 16 == 0)
+            units_of_x[c * blocks + k8 / 16] =
+                __uint_as_float(top >= 0x7f800000u ? 0x7fc00000u : static_cast<uint32_t>(unit_exp - 4) << 23);
+          constexpr unsigned kPer = kFmt / 8;  // pieces per group
+          const unsigned in = k8 % kPer;
+          at = k8 - in + (in % F::kWords) * 4 + in / F::kWords;  // group | quarter | word -> group | word | quarter
+          v[b] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
+        }
+        *reinterpret_cast<uint4*>(xs + static_cast<size_t>(c) * x_bytes + at * 16) = v[b];
+      }
     }
   };
   int item_index = begin / per_item, unit = begin - item_index * per_item;
@@ -341,11 +439,23 @@ __global__ void __launch_bounds__(kThreads, 2) skinny_kernel(const SkinnyArgs a)
   __syncthreads();
   // Columns past the item's last read its last one again: their sums are never used.
   const uint8_t* xcol[NT];
+  const float* units_at[NT][2];  // of the columns whose sums this lane gets (packed: one)
   auto point_x = [&] {
+    const int last = item.count - 1;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) xcol[n] = xs + static_cast<size_t>(min(n * 8 + g, item.count - 1)) * x_bytes + q * 16;
+    for (int n = 0; n < NT; ++n) {
+      const int c = kPacked ? g >> 1 : n * 8 + g;
+      xcol[n] = xs + static_cast<size_t>(min(c, last)) * x_bytes + q * 16 + (kPacked ? (g & 1) * 8 : 0);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) units_at[n][j] = units_of_x + min(kPacked ? q : n * 8 + 2 * q + j, last) * blocks;
+    }
   };
   point_x();
+  // start of every group's sums; opaque, so that it stays in registers
+  int4 start;
+  asm volatile("mov.b32 %0, %4;\n\tmov.b32 %1, %4;\n\tmov.b32 %2, %4;\n\tmov.b32 %3, %4;"
+               : "=r"(start.x), "=r"(start.y), "=r"(start.z), "=r"(start.w)
+               : "n"(kFloatBias));
 
   float acc[NT][4];
 #pragma unroll
@@ -353,72 +463,147 @@ __global__ void __launch_bounds__(kThreads, 2) skinny_kernel(const SkinnyArgs a)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
 
-  int units_left = end - begin, i = 0, buffer = 0;
+  int units_left = end - begin, i = 0, buffer = 0, slot = 0;
+  auto point_scales = [&] {
+    if constexpr (kFmt != 0) {
+      const int base = (unit * tiles_at_once + rt) * kOut;
+      const int ra = min(base + g, a.rows - 1);
+      const int rb = kGateUp ? ra : min(base + g + 8, a.rows - 1);
+      const size_t from = static_cast<size_t>(routed ? item.expert : 0) * a.s_expert;
+      const uint16_t* second = kGateUp ? a.s1 : a.s0;
+      odd_a = reinterpret_cast<uintptr_t>(a.s0 + from + static_cast<size_t>(ra) * row_groups) >> 1 & 1;
+      odd_b = reinterpret_cast<uintptr_t>(second + from + static_cast<size_t>(rb) * row_groups) >> 1 & 1;
+    }
+  };
+  point_scales();
   while (true) {
+    const int step = i * a.k_warps + kw;
+    wait_copies<kDepth - 1>();
+    __syncwarp();  // the scales were fetched by other lanes
+    if (step < steps) {
+      const uint8_t* at = ring + slot * F::kSlot;
+      const uint8_t* x_at[NT];
 #pragma unroll
-    for (int d = 0; d < kDepth; ++d) {
-      const Piece va = pa[d], vb = pb[d];
-      const int step = i * a.k_warps + kw;
-      if (step < steps) {
+      for (int n = 0; n < NT; ++n) x_at[n] = xcol[n] + step * (F::kStep * 2);
+      uint32_t sa[F::kScaleWords + 1], sb[F::kScaleWords + 1];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int x_at = (step * 2 + h) * (F::kHalf * 2);
-          const uint32_t aw[4] = {va.w[h].x, va.w[h].y, va.w[h].z, va.w[h].w};
-          const uint32_t bw[4] = {vb.w[h].x, vb.w[h].y, vb.w[h].z, vb.w[h].w};
-          if constexpr (kFmt == 0) {
+      for (int j = 0; j < F::kScaleWords; ++j) {
+        sa[j] = *reinterpret_cast<const uint32_t*>(at + F::kScaleAt + j * 64 + g * 4);
+        sb[j] = *reinterpret_cast<const uint32_t*>(at + F::kScaleAt + j * 64 + 32 + g * 4);
+      }
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const uint4 x4 = *reinterpret_cast<const uint4*>(xcol[n] + x_at);
-              mma_bf16(acc[n], aw[0], bw[0], aw[1], bw[1], x4.x, x4.y);
-              mma_bf16(acc[n], aw[2], bw[2], aw[3], bw[3], x4.z, x4.w);
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* ra = at + h * F::kHalfBytes + g * F::kRow;
+        const uint8_t* rb = ra + 8 * F::kRow;
+        if constexpr (kFmt == 0) {
+          const uint4 u = *reinterpret_cast<const uint4*>(ra + q * 16), v = *reinterpret_cast<const uint4*>(rb + q * 16);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint4 x4 = *reinterpret_cast<const uint4*>(x_at[n] + h * (F::kHalf * 2));
+            mma_bf16(acc[n], u.x, v.x, u.y, v.y, x4.x, x4.y);
+            mma_bf16(acc[n], u.z, v.z, u.w, v.w, x4.z, x4.w);
+          }
+        } else {
+          uint32_t aw[4], bw[4];  // words of group 0, then of group 1, ..
+          if constexpr (kFmt == 128) {
+            const uint4 u = *reinterpret_cast<const uint4*>(ra + q * 16), v = *reinterpret_cast<const uint4*>(rb + q * 16);
+            aw[0] = u.x, aw[1] = u.y, aw[2] = u.z, aw[3] = u.w;
+            bw[0] = v.x, bw[1] = v.y, bw[2] = v.z, bw[3] = v.w;
+          } else if constexpr (kFmt == 64) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const uint2 u = *reinterpret_cast<const uint2*>(ra + s * 32 + q * 8);
+              const uint2 v = *reinterpret_cast<const uint2*>(rb + s * 32 + q * 8);
+              aw[2 * s] = u.x, aw[2 * s + 1] = u.y;
+              bw[2 * s] = v.x, bw[2 * s + 1] = v.y;
             }
           } else {
 #pragma unroll
-            for (int s = 0; s < F::kGroups; ++s) {
-              float sum[NT][4];
-              const int group = (step * 2 + h) * F::kGroups + s;
+            for (int s = 0; s < 4; ++s) {
+              aw[s] = *reinterpret_cast<const uint32_t*>(ra + s * 16 + q * 4);
+              bw[s] = *reinterpret_cast<const uint32_t*>(rb + s * 16 + q * 4);
+            }
+          }
+          // scale of group s of this half, of a row whose first is the low or (odd) the high half of word 0
+          auto scale_of = [&](const uint32_t* words, uint32_t odd, int s) {
+            const int gi = h * F::kGroups + s;
+            const uint32_t v = __funnelshift_r(words[gi >> 1], words[(gi >> 1) + 1], odd * 16);
+            return __uint_as_float(gi & 1 ? v & 0xffff0000u : v << 16);
+          };
+          const Two bias = two(-kFloatBiasValue, -kFloatBiasValue), high_weight = two(256.0f, 256.0f);
+          Two block_a[NT], block_b[NT];  // the block's sums over groups, rows g and g + 8
+          float block_p[2] = {0.f, 0.f};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) block_a[n] = block_b[n] = two(0.f, 0.f);
+#pragma unroll
+          for (int s = 0; s < F::kGroups; ++s) {
+            int4 high[NT], low[NT];
+#pragma unroll
+            for (int w = 0; w < F::kWords; ++w) {
+              const uint32_t u = aw[s * F::kWords + w], v = bw[s * F::kWords + w];
+              const uint32_t a0 = (u << 4 & 0xf0f0f0f0u) ^ 0x80808080u, a1 = (v << 4 & 0xf0f0f0f0u) ^ 0x80808080u;
+              const uint32_t a2 = (u & 0xf0f0f0f0u) ^ 0x80808080u, a3 = (v & 0xf0f0f0f0u) ^ 0x80808080u;
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                const float2 start = *reinterpret_cast<const float2*>(sums + group * kCols + n * 8 + 2 * q);
-                sum[n][0] = sum[n][2] = start.x;
-                sum[n][1] = sum[n][3] = start.y;
-              }
-#pragma unroll
-              for (int w = 0; w < F::kWords; ++w) {
-                const uint32_t u = aw[s * F::kWords + w], v = bw[s * F::kWords + w];
-                const uint32_t a0 = codes(u, 0), a1 = codes(u, 1), a2 = codes(u, 2), a3 = codes(u, 3);
-                const uint32_t b0 = codes(v, 0), b1 = codes(v, 1), b2 = codes(v, 2), b3 = codes(v, 3);
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                  const uint4 x4 = *reinterpret_cast<const uint4*>(xcol[n] + x_at + (s * F::kWords + w) * 64);
-                  mma_bf16(sum[n], a0, b0, a1, b1, x4.x, x4.y);
-                  mma_bf16(sum[n], a2, b2, a3, b3, x4.z, x4.w);
+                const uint8_t* from = x_at[n] + h * (F::kHalf * 2) + (s * F::kWords + w) * 64;
+                if constexpr (kPacked) {
+                  const uint2 x2 = *reinterpret_cast<const uint2*>(from);
+                  mma_bytes(high[n], w == 0 ? start : high[n], a0, a1, a2, a3, x2.x, x2.y);
+                } else {
+                  const uint4 x4 = *reinterpret_cast<const uint4*>(from);
+                  mma_bytes(high[n], w == 0 ? start : high[n], a0, a1, a2, a3, x4.x, x4.y);
+                  mma_bytes(low[n], w == 0 ? start : low[n], a0, a1, a2, a3, x4.z, x4.w);
                 }
               }
-              const float fa = scale_of(va, h * F::kGroups + s), fb = scale_of(vb, h * F::kGroups + s);
+            }
+            const float fa = scale_of(sa, odd_a, s), fb = scale_of(sb, odd_b, s);
+            if constexpr (kPacked) {
+              const float2 va = split(add(two(high[0].x, high[0].y), bias)), vb = split(add(two(high[0].z, high[0].w), bias));
+              block_p[0] = fmaf(fa, fmaf(va.x, 256.0f, va.y), block_p[0]);
+              block_p[1] = fmaf(fb, fmaf(vb.x, 256.0f, vb.y), block_p[1]);
+            } else {
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                acc[n][0] += fa * sum[n][0];
-                acc[n][1] += fa * sum[n][1];
-                acc[n][2] += fb * sum[n][2];
-                acc[n][3] += fb * sum[n][3];
+                const Two sum_a = fma(add(two(high[n].x, high[n].y), bias), high_weight, add(two(low[n].x, low[n].y), bias));
+                const Two sum_b = fma(add(two(high[n].z, high[n].w), bias), high_weight, add(two(low[n].z, low[n].w), bias));
+                block_a[n] = fma(two(fa, fa), sum_a, block_a[n]);
+                block_b[n] = fma(two(fb, fb), sum_b, block_b[n]);
               }
+            }
+          }
+          const int block = step * 2 + h;
+          if constexpr (kPacked) {
+            const float unit = units_at[0][0][block];
+            acc[0][0] = fmaf(unit, block_p[0], acc[0][0]);
+            acc[0][2] = fmaf(unit, block_p[1], acc[0][2]);
+          } else {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const Two ux = two(units_at[n][0][block], units_at[n][1][block]);
+              const float2 ra2 = split(fma(ux, block_a[n], two(acc[n][0], acc[n][1])));
+              const float2 rb2 = split(fma(ux, block_b[n], two(acc[n][2], acc[n][3])));
+              acc[n][0] = ra2.x, acc[n][1] = ra2.y;
+              acc[n][2] = rb2.x, acc[n][3] = rb2.y;
             }
           }
         }
       }
-      issue(d);
-      if (++i < per_warp) continue;
-
+    }
+    __syncwarp();  // every lane has read the slot
+    issue();
+    slot = slot + 1 == kDepth ? 0 : slot + 1;
+    if (++i == per_warp) {
       // ---- end of the unit: add the sums of each tile's warps (in warp order) and write
       i = 0;
-      float* mine = part + ((buffer * kWarps + warp) * kCols + 2 * q) * 16 + g;
+      float* mine = part + ((buffer * kWarps + warp) * kCols + (kPacked ? q : 2 * q)) * 16 + g;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         mine[n * 128] = acc[n][0];
-        mine[n * 128 + 16] = acc[n][1];
         mine[n * 128 + 8] = acc[n][2];
-        mine[n * 128 + 24] = acc[n][3];
+        if constexpr (!kPacked) {
+          mine[n * 128 + 16] = acc[n][1];
+          mine[n * 128 + 24] = acc[n][3];
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
       }
@@ -431,7 +616,9 @@ __global__ void __launch_bounds__(kThreads, 2) skinny_kernel(const SkinnyArgs a)
         if (c >= item.count || row >= a.rows) continue;
         const float* from = all + (t * a.k_warps * kCols + c) * 16 + r;
         float v = 0.f, u = 0.f;
-        for (int w = 0; w < a.k_warps; ++w) {
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          if (w >= a.k_warps) break;
           v += from[w * kCols * 16];
           if constexpr (kGateUp) u += from[w * kCols * 16 + 8];
         }
@@ -442,7 +629,10 @@ __global__ void __launch_bounds__(kThreads, 2) skinny_kernel(const SkinnyArgs a)
         else
           static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
       }
-      buffer ^= 1;
+      if constexpr (part_buffers(kWarps) == 2)
+        buffer ^= 1;
+      else
+        __syncthreads();
       if (--units_left == 0) return;
       if (++unit == per_item) {  // the next item's x rows; every warp has used the old ones
         unit = 0;
@@ -451,6 +641,7 @@ __global__ void __launch_bounds__(kThreads, 2) skinny_kernel(const SkinnyArgs a)
         __syncthreads();
         point_x();
       }
+      point_scales();
     }
   }
 }
@@ -496,56 +687,89 @@ cudaError_t launch_kernel(K kernel, dim3 grid, int threads, size_t smem, bool de
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
-template <int kFmt, bool kGateUp, int NT, bool kOutF32>
-cudaError_t launch_tile(SkinnyArgs a, cudaStream_t stream) {
+template <int kFmt>
+size_t smem_bytes(const SkinnyArgs& a, int warps) {
+  const int step = Format<kFmt>::kStep;
+  const int padded = (a.k + step - 1) / step * step;
+  const bool routed = a.indices != nullptr;
+  return carve_smem(warps, Format<kFmt>::kSlot, a.cols, padded, kFmt == 0 ? 0 : padded / 128, routed ? a.pairs : 0)
+      .total;
+}
+
+template <int kFmt, bool kGateUp, int kCols, bool kOutF32, int kWarps>
+cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream);
+
+// Eight warps a CTA and two CTAs an SM; where x rows leave room for one, sixteen warps if they fit.
+template <int kFmt, bool kGateUp, int kCols, bool kOutF32>
+cudaError_t launch_tile(const SkinnyArgs& a, cudaStream_t stream) {
+  const size_t two = smem_bytes<kFmt>(a, 8), one = smem_bytes<kFmt>(a, 16);
+  return 2 * (two + 1024) > kSmemPerSm && one <= kMaxSmem ? launch_warps<kFmt, kGateUp, kCols, kOutF32, 16>(a, stream)
+                                                          : launch_warps<kFmt, kGateUp, kCols, kOutF32, 8>(a, stream);
+}
+
+template <int kFmt, bool kGateUp, int kCols, bool kOutF32, int kWarps>
+cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
+  const auto kernel = skinny_kernel<kFmt, kGateUp, kCols, kOutF32, kWarps>;
   const int step = Format<kFmt>::kStep;
   const int steps = (a.k + step - 1) / step;
   const bool routed = a.indices != nullptr;
-  const SkinnySmem lay = carve_smem(a.cols, steps * step, kFmt == 0 ? 0 : steps * step / (kFmt == 0 ? 1 : kFmt),
-                                    routed ? a.pairs : 0, routed ? a.experts : 0);
-  if (lay.total > kMaxSmem) return cudaErrorInvalidValue;
+  const size_t smem = smem_bytes<kFmt>(a, kWarps);
+  if (smem > kMaxSmem) return cudaErrorInvalidValue;
   static PerDeviceOnce attr;
-  cudaError_t err = attr.run([] {
-    return cudaFuncSetAttribute(skinny_kernel<kFmt, kGateUp, NT, kOutF32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kMaxSmem);
-  });
+  cudaError_t err =
+      attr.run([&] { return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmem); });
   if (err != cudaSuccess) return err;
   const int items = routed ? a.pairs : (a.tokens + a.cols - 1) / a.cols;
-  const int slots = device_sm_count() * (lay.total <= kTwoCtaSmem ? 2 : 1);
-  auto units = [&](int k_warps) {
-    const int rows = (kGateUp ? 8 : 16) * (kWarps / k_warps);
-    return static_cast<long long>(items) * ((a.rows + rows - 1) / rows);
-  };
-  // All warps to a tile, unless that leaves a warp fewer than 4 steps a tile and there are tiles
-  // enough: the barrier and the additions at a tile's end then cost as much as its products.
-  a.k_warps = kWarps;
-  while (a.k_warps > 2 && steps < 4 * a.k_warps && units(a.k_warps / 2) >= 2 * slots) a.k_warps /= 2;
-  const long long most = units(a.k_warps);
+  const int slots = device_sm_count() * (kWarps == 8 && 2 * (smem + 1024) <= kSmemPerSm ? 2 : 1);
+  // Warps to a tile: a unit costs its steps per warp and about 1.5 more for the barrier and the additions at
+  // its end, and the CTA with the most units decides. (On 16384 x 8192 at 7 columns 2 warps take 24.4 us and
+  // 16 take 29.0.) With routing the expected number of experts stands for the items.
+  const double likely = routed ? a.experts * (1.0 - std::exp(-static_cast<double>(a.pairs) / a.experts)) : 0.0;
+  const long long expected = routed ? static_cast<long long>(likely) + 1 : items;
+  long long best = 0;
+  for (int k = 1; k <= kWarps; k *= 2) {
+    const int rows = (kGateUp ? 8 : 16) * (kWarps / k);
+    const long long n = expected * ((a.rows + rows - 1) / rows);
+    const long long cost = (n + slots - 1) / slots * (2 * ((steps + k - 1) / k) + 3);
+    if (best == 0 || cost < best) {
+      best = cost;
+      a.k_warps = k;
+    }
+  }
+  const int unit_rows = (kGateUp ? 8 : 16) * (kWarps / a.k_warps);
+  const long long most = static_cast<long long>(items) * ((a.rows + unit_rows - 1) / unit_rows);
   const int grid = static_cast<int>(most < slots ? most : slots);
-  return launch_kernel(skinny_kernel<kFmt, kGateUp, NT, kOutF32>, dim3(grid), kThreads, lay.total, a.dependent != 0,
-                       stream, a);
+  return launch_kernel(kernel, dim3(grid), 32 * kWarps, smem, a.dependent != 0, stream, a);
+}
+
+template <int kFmt, bool kGateUp, bool kOutF32>
+cudaError_t launch_columns(const SkinnyArgs& a, cudaStream_t stream) {
+  if constexpr (kFmt != 0)
+    if (a.cols <= 4) return launch_tile<kFmt, kGateUp, 4, kOutF32>(a, stream);
+  return a.cols <= 8 ? launch_tile<kFmt, kGateUp, 8, kOutF32>(a, stream)
+                     : launch_tile<kFmt, kGateUp, 16, kOutF32>(a, stream);
 }
 
 template <bool kGateUp, bool kOutF32>
 cudaError_t launch_format(const SkinnyArgs& a, int group, cudaStream_t stream) {
-  const bool wide = a.cols > 8;
   switch (group) {
-    case 0: return wide ? launch_tile<0, kGateUp, 2, kOutF32>(a, stream) : launch_tile<0, kGateUp, 1, kOutF32>(a, stream);
-    case 32: return wide ? launch_tile<32, kGateUp, 2, kOutF32>(a, stream) : launch_tile<32, kGateUp, 1, kOutF32>(a, stream);
-    case 64: return wide ? launch_tile<64, kGateUp, 2, kOutF32>(a, stream) : launch_tile<64, kGateUp, 1, kOutF32>(a, stream);
-    case 128:
-      return wide ? launch_tile<128, kGateUp, 2, kOutF32>(a, stream) : launch_tile<128, kGateUp, 1, kOutF32>(a, stream);
+    case 0: return launch_columns<0, kGateUp, kOutF32>(a, stream);
+    case 32: return launch_columns<32, kGateUp, kOutF32>(a, stream);
+    case 64: return launch_columns<64, kGateUp, kOutF32>(a, stream);
+    case 128: return launch_columns<128, kGateUp, kOutF32>(a, stream);
   }
   return cudaErrorInvalidValue;
 }
 
 }  // namespace
 
-int skinny_columns(int want, int k, int group, int pairs, int experts) {
+int skinny_columns(int want, int k, int group, int pairs) {
   const int step = group == 0 ? Format<0>::kStep : Format<32>::kStep;
+  const int slot = group == 0 ? Format<0>::kSlot : group == 128 ? Format<128>::kSlot : group == 64 ? Format<64>::kSlot : Format<32>::kSlot;
   const int padded = (k + step - 1) / step * step;
   int cols = want < kSkinnyMaxColumns ? want : kSkinnyMaxColumns;
-  while (cols > 0 && carve_smem(cols, padded, group == 0 ? 0 : padded / group, pairs, experts).total > kMaxSmem) --cols;
+  while (cols > 0 && carve_smem(8, slot, cols, padded, group == 0 ? 0 : padded / 128, pairs).total > kMaxSmem)
+    --cols;
   return cols;
 }
 

@@ -28,15 +28,16 @@ def _rows_ok(x: torch.Tensor) -> bool:
 
 def _validate(x, gate_proj, up_proj, down_proj) -> _lib.FfnShape:
     _check(x.is_cuda, "x must be a CUDA tensor")
-    _check(x.dim() == 2 and x.dtype == _BF16, "x must be [T, H] bf16")
+    _check(x.dim() == 2 and x.dtype is _BF16, "x must be [T, H] bf16")
     T, H = x.shape
-    for name, w in (("gate_proj", gate_proj), ("up_proj", up_proj), ("down_proj", down_proj)):
-        _check(w.device == x.device, f"{name} must be on {x.device}")
-        _check(w.dim() == 2 and w.dtype == _BF16, f"{name} must be 2-D bf16")
-        _check(w.is_contiguous(), f"{name} must be contiguous")
+    dev = x.device
+    for w in (gate_proj, up_proj, down_proj):
+        if not (w.device == dev and w.dtype is _BF16 and w.is_contiguous()):
+            raise RuntimeError(f"gate_proj, up_proj and down_proj must be contiguous bf16 on {dev}")
+    _check(gate_proj.dim() == 2, "gate_proj must be [F, H]")
     F = gate_proj.shape[0]
-    _check(gate_proj.shape[1] == H and up_proj.shape == gate_proj.shape, "gate_proj and up_proj must be [F, H]")
-    _check(down_proj.shape[0] == H and down_proj.shape[1] == F, "down_proj must be [H, F]")
+    _check(gate_proj.shape == (F, H) and up_proj.shape == (F, H), "gate_proj and up_proj must be [F, H]")
+    _check(down_proj.shape == (H, F), "down_proj must be [H, F]")
     _check(H > 0 and F > 0 and H % 8 == 0 and F % 8 == 0, "H and F must be multiples of 8")
     _check(_rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least H) apart")
     return _lib.FfnShape(T, H, F)
@@ -46,25 +47,32 @@ def _stride(x: torch.Tensor) -> int:
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+# The current stream's handle; the public call builds a Stream object first, 2 us of a 10 us call.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(device: torch.device, name: str, *args) -> None:
     """Calls a C-ABI entry, whose last argument is the stream, with `device` current."""
     fn = getattr(_lib.load(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, name)
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
 def _forward(x, gate_proj, up_proj, down_proj) -> torch.Tensor:
     shape = _validate(x, gate_proj, up_proj, down_proj)
-    out = torch.empty((shape.tokens, shape.hidden), dtype=_BF16, device=x.device)
+    out = x.new_empty((shape.tokens, shape.hidden))
     if shape.tokens == 0:
         return out
     n = ctypes.c_size_t(0)
     _lib.check(_lib.load().cernels_gated_ffn_workspace_bytes(ctypes.byref(shape), 0, ctypes.byref(n)), "workspace query")
-    ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty((n.value + 1) // 2)
     _call(x.device, "cernels_gated_ffn", ctypes.byref(shape), x.data_ptr(), _stride(x), gate_proj.data_ptr(),
           up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), ws.data_ptr(), n.value)
     return out
@@ -75,8 +83,8 @@ class _GatedFfn(torch.autograd.Function):
     def forward(ctx, x, gate_proj, up_proj, down_proj):
         shape = _validate(x, gate_proj, up_proj, down_proj)
         T, F, dev = shape.tokens, shape.intermediate, x.device
-        out = torch.empty((T, shape.hidden), dtype=_BF16, device=dev)
-        act = torch.empty((T, F), dtype=_BF16, device=dev)
+        out = x.new_empty((T, shape.hidden))
+        act = x.new_empty((T, F))
         n = ctypes.c_size_t(0)
         _lib.check(_lib.load().cernels_gated_ffn_saved_bytes(ctypes.byref(shape), ctypes.byref(n)), "size query")
         saved = torch.empty(n.value // 4, dtype=torch.float32, device=dev)
@@ -85,27 +93,36 @@ class _GatedFfn(torch.autograd.Function):
                   gate_proj.data_ptr(), up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), act.data_ptr(),
                   saved.data_ptr())
         ctx.save_for_backward(x, gate_proj, up_proj, down_proj, act, saved)
+        ctx.shape = shape
         return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        x, gate_proj, up_proj, down_proj, act, saved = ctx.saved_tensors
-        shape = _lib.FfnShape(x.shape[0], x.shape[1], gate_proj.shape[0])
-        dev = x.device
-        dout = dout.contiguous()
-        if dout.data_ptr() % 16:
-            dout = dout.clone()
-        grads = [torch.empty(t.shape, dtype=_BF16, device=dev) if need else None
-                 for t, need in zip((x, gate_proj, up_proj, down_proj), ctx.needs_input_grad)]
-        n = ctypes.c_size_t(0)
-        _lib.check(_lib.load().cernels_gated_ffn_workspace_bytes(ctypes.byref(shape), 1, ctypes.byref(n)),
-                   "workspace query")
-        ws = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        _call(dev, "cernels_gated_ffn_backward", ctypes.byref(shape), x.data_ptr(), _stride(x), gate_proj.data_ptr(),
-              up_proj.data_ptr(), down_proj.data_ptr(), act.data_ptr(), saved.data_ptr(), dout.data_ptr(),
-              *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), n.value)
-        return tuple(grads)
+        # Gradients of gradients are refused; the wrapper that sees to that is only needed, and only
+        # paid for, where the caller records the backward pass.
+        return (_backward_recorded if torch.is_grad_enabled() else _backward)(ctx, dout)
+
+
+def _backward(ctx, dout):
+    x, gate_proj, up_proj, down_proj, act, saved = ctx.saved_tensors
+    shape = ctx.shape
+    dev = x.device
+    dout = dout.contiguous()
+    if dout.data_ptr() % 16:
+        dout = dout.clone()
+    grads = [dout.new_empty(t.shape) if need else None
+             for t, need in zip((x, gate_proj, up_proj, down_proj), ctx.needs_input_grad)]
+    n = ctypes.c_size_t(0)
+    _lib.check(_lib.load().cernels_gated_ffn_workspace_bytes(ctypes.byref(shape), 1, ctypes.byref(n)),
+               "workspace query")
+    ws = dout.new_empty((n.value + 1) // 2)
+    _call(dev, "cernels_gated_ffn_backward", ctypes.byref(shape), x.data_ptr(), _stride(x), gate_proj.data_ptr(),
+          up_proj.data_ptr(), down_proj.data_ptr(), act.data_ptr(), saved.data_ptr(), dout.data_ptr(),
+          *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), n.value)
+    return tuple(grads)
+
+
+_backward_recorded = once_differentiable(_backward)
 
 
 def gated_ffn(x: torch.Tensor, gate_proj: torch.Tensor, up_proj: torch.Tensor, down_proj: torch.Tensor) -> torch.Tensor:

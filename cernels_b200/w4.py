@@ -39,31 +39,34 @@ def quantize_w4(weight: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, t
 
 
 def _check_no_grad(*tensors: torch.Tensor) -> None:
-    _check(not (torch.is_grad_enabled() and any(t.requires_grad for t in tensors)),
-           "4-bit products have no gradient: call them under torch.no_grad()")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            _check(not t.requires_grad, "4-bit products have no gradient: call them under torch.no_grad()")
 
 
 def _check_w4(name: str, q: torch.Tensor, s: torch.Tensor, lead: tuple, k: int, dev: torch.device) -> int:
     """The group size of codes q [*lead, k / 2] with scales s [*lead, k / G]."""
-    _check(q.device == dev and s.device == dev, f"{name} must be on {dev}")
-    _check(q.dtype == torch.uint8 and s.dtype == _BF16, f"{name}: codes must be uint8 and scales bf16")
-    _check(q.is_contiguous() and s.is_contiguous(), f"{name} must be contiguous")
-    _check(tuple(q.shape) == (*lead, k // 2) and k % 2 == 0, f"{name}: codes must be {[*lead, k // 2]}")
-    _check(tuple(s.shape[:-1]) == lead and s.shape[-1] > 0, f"{name}: scales must be {[*lead, 'K / group']}")
-    group = k // s.shape[-1]
-    _check(group in GROUPS and group * s.shape[-1] == k, f"{name}: group must be one of {GROUPS} and divide K")
+    if not (q.device == dev and s.device == dev and q.dtype is torch.uint8 and s.dtype is _BF16
+            and q.is_contiguous() and s.is_contiguous()):
+        raise RuntimeError(f"{name} must be contiguous uint8 codes and bf16 scales on {dev}")
+    n_groups = s.shape[-1]
+    if k % 2 or q.shape != (*lead, k // 2) or s.shape != (*lead, n_groups) or n_groups == 0:
+        raise RuntimeError(f"{name}: codes must be {[*lead, k // 2]} and scales {[*lead, 'K / group']}")
+    group = k // n_groups
+    if group not in GROUPS or group * n_groups != k:
+        raise RuntimeError(f"{name}: group must be one of {GROUPS} and divide K")
     return group
 
 
 def _linear_w4(x, qweight, scales):
     _check(x.is_cuda, "x must be a CUDA tensor")
-    _check(x.dim() == 2 and x.dtype == _BF16, "x must be [T, K] bf16")
-    _check(qweight.dim() == 2 and scales.dim() == 2, "qweight must be [N, K / 2] and scales [N, K / group]")
+    _check(x.dim() == 2 and x.dtype is _BF16, "x must be [T, K] bf16")
+    _check(qweight.dim() == 2, "qweight must be [N, K / 2]")
     T, K = x.shape
     N = qweight.shape[0]
     group = _check_w4("qweight", qweight, scales, (N,), K, x.device)
     _check(_rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least K) apart")
-    out = torch.empty((T, N), dtype=_BF16, device=x.device)
+    out = x.new_empty((T, N))
     if T and N:
         _call(x.device, "cernels_linear_w4", T, N, K, group, x.data_ptr(), _stride(x), qweight.data_ptr(),
               scales.data_ptr(), out.data_ptr())
@@ -91,14 +94,14 @@ def _moe_experts_decode_w4(x, gate_up_q, gate_up_scales, down_q, down_scales, in
         _check(t.device == x.device and t.dtype == dtype and t.is_contiguous() and tuple(t.shape) == (T, topk),
                f"{name} must be contiguous [T, topk] {dtype} on {x.device}")
     _check(T * topk <= DECODE_MAX_PAIRS, f"at most {DECODE_MAX_PAIRS} (token, slot) pairs per call")
-    out = torch.empty_like(x)
+    out = x.new_empty((T, H))
     if T == 0:
         return out
     shape = _lib.MoeShape(T, H, E, F, topk, _lib.LAYOUT_LINEAR)
     n = ctypes.c_size_t(0)
     _lib.check(_lib.load().cernels_moe_w4_workspace_bytes(ctypes.byref(shape), group, ctypes.byref(n)),
                "workspace query")
-    ws = torch.empty(n.value, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty((n.value + 1) // 2)
     _call(x.device, "cernels_moe_experts_decode_w4", ctypes.byref(shape), group, x.data_ptr(), gate_up_q.data_ptr(),
           gate_up_scales.data_ptr(), down_q.data_ptr(), down_scales.data_ptr(), indices.data_ptr(), weights.data_ptr(),
           out.data_ptr(), ws.data_ptr(), n.value)

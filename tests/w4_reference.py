@@ -1,10 +1,10 @@
 """4-bit products in 64 bits, with bounds of their errors (the constants of ffn_reference).
 
-Codes and scales are exact in 64 bits and never rounded by the operator, so a linear layer's error is
-its 32-bit sums' and the output's rounding. The operator sums (128 + q) x within a group of G, from a
-start of -136 sum(x), to get the sum of (q - 8) x: G + 3 roundings of at most 2^-23 of magnitudes that
-add up to (143 + 136) sum|x|; then the K / G groups' sums times their scales, with two roundings each.
-The experts' call adds the rounding of the halved product, as an operand.
+Codes and scales are exact in 64 bits and never rounded by the operator. It takes x as 14 bits and a
+sign below the largest value of each block of 128, rounding it by at most 2^-14 of that value; sums
+within a group are exact integers, and each group's sum then meets seven 32-bit roundings on its way
+into its block's and the row's sum (conversion, two for its parts, scale, unit, two additions), which add up with
+the number of groups. The experts' call adds the rounding of the halved product, as an operand.
 """
 
 import torch
@@ -27,11 +27,12 @@ def values(q, s):
 
 
 def _sum_bound(x, q, s):
-    """Bound of the 32-bit sums of |x| [T, K] with the weights of (q, s) [N, ..]."""
-    groups = s.shape[-1]
-    G = x.shape[1] // groups
-    inside = (G + 3) * ADD * 279 * (x.unflatten(1, (groups, G)).sum(-1) @ s.double().abs().T)
-    return inside + (groups + 2) * ADD * (x @ values(q, s).abs().T + inside)
+    """Bound of the operator's sums of |x| [T, K] with the weights of (q, s) [N, ..]."""
+    w = values(q, s).abs()
+    pad = -x.shape[1] % 128
+    xb, wb = (torch.nn.functional.pad(v, (0, pad)).unflatten(1, (-1, 128)) for v in (x, w))
+    rounded = 2.0 ** -14 * (xb.amax(-1) @ wb.sum(-1).T)
+    return rounded + (s.shape[-1] + 7) * ADD * (x @ w.T + rounded)
 
 
 def linear(x, q, s):
