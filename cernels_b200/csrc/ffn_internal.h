@@ -6,6 +6,29 @@
 
 namespace cernels {
 
+#ifdef __CUDACC__
+// Programmatic dependent launch: a kernel launched as the dependent of the one before it on its
+// stream may start while that one runs, and waits here for its end before it touches its results. Every
+// CTA of a dependent kernel waits, so that its own end implies the other's.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class K, class... A>
+cudaError_t launch_kernel(K kernel, dim3 grid, int threads, size_t smem, bool dependent, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+#endif
+
 // ---- pair_gemm.cu: bf16 matrix products over CTA pairs (more than a few tokens, and training)
 struct FfnShape {
   int tokens, hidden, inter;

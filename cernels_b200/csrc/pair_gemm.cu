@@ -22,6 +22,9 @@
 // 4 H F operations a token against 16 F bytes of traffic, more for H above about 1000, and
 // rounding them to bf16 would add its error to every gradient. h, dg and du are rounded to bf16,
 // once each: they are operands of the next product.
+#include <algorithm>
+#include <cmath>
+
 #include "ffn_internal.h"
 #include "pair_gemm.cuh"
 
@@ -75,6 +78,7 @@ struct PairArgs {
   float* gate_up;  // stored products (kGateUp writes when not null, kGradGateUp reads)
   int inter;       // F
   int row_blocks;  // ceil(T / 32)
+  int dependent;   // operands are written by the kernel launched just before on this stream
   unsigned long long wait_ns;
 };
 
@@ -146,6 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
+  let_next_kernel_start();
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
@@ -174,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   pair_sync();  // both CTAs' barriers exist before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  if (args.dependent) wait_for_previous_kernel();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA loads
@@ -290,13 +296,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
       const int acc = local & 1;
       const int row0 = c.m_tile * 2 * kBM + static_cast<int>(rank) * kBM + quarter * 32;
       const size_t row_block = static_cast<size_t>(row0 >> 5);
-      if constexpr (kEpi == kGradGateUp) {
-        // this warp's part of the stored products is one contiguous run: into L2 during the MMAs
-        const int f0 = c.n_tile * BN + half * (BN / 2);
-        const int cols = min(BN / 2, args.inter - f0);
-        if (lane == 0 && cols > 0 && row_block < static_cast<size_t>(args.row_blocks))
-          bulk_prefetch_l2(saved + ((row_block * (args.inter >> 2) + (f0 >> 2)) << 6), static_cast<uint32_t>(cols) * 256);
-      }
       if (!mbar_wait_bounded(&tfull_bar[acc], (local >> 1) & 1, &g_ffn_status, kStatusTimeoutEpilogue, abort_flag,
                              args.wait_ns))
         break;
@@ -474,8 +473,19 @@ cudaError_t launch(Builder& b, cudaStream_t stream) {
   const int pairs = b.args.total_tiles < max_pairs ? b.args.total_tiles : max_pairs;
   if (pairs <= 0) return cudaSuccess;
   b.args.wait_ns = wait_limit_ns(kWaitLimitNs);
-  pair_gemm_kernel<kEpi, BN><<<2 * pairs, kThreads, C::kSmem, stream>>>(b.maps, b.args);
-  return cudaGetLastError();
+  return launch_kernel(pair_gemm_kernel<kEpi, BN>, dim3(2 * pairs), kThreads, C::kSmem, b.args.dependent != 0, stream, b.maps,
+                       b.args);
+}
+
+int tiles_of(int m, int n, int tile_n) { return (m + 2 * kBM - 1) / (2 * kBM) * ((n + tile_n - 1) / tile_n); }
+
+// Whether 128-wide tiles beat 256-wide ones for `wide` and `narrow` tiles of each: a launch takes as many
+// rounds as its fullest pair has tiles, and a 128-wide tile costs 0.75 of a 256-wide one: both are bound by the
+// 64 bytes a cycle that an SM gets from L2, and it needs 24 KB per K block instead of 32. (Forward at T = 301,
+// H = 2048, F = 768: 18.9 us with 128, 24.9 with 256; at T = 4096, F = 1408: 65.0 and 56.4.)
+bool narrow_tiles(double wide, double narrow) {
+  const int pairs = device_sm_count() / 2;
+  return std::ceil(narrow / pairs) * 0.75 < std::ceil(wide / pairs);
 }
 
 template <int BN>
@@ -503,6 +513,7 @@ cudaError_t down_product(const FfnShape& s, const __nv_bfloat16* h, const __nv_b
   p.a_map[0] = b.k_major(h, s.tokens, s.inter, s.inter, kBM);
   p.b_map[0] = b.k_major(down, s.hidden, s.inter, s.inter, BN / 2);
   p.out_map[0] = b.output(out, s.tokens, s.hidden);
+  b.args.dependent = 1;
   return launch<kPlain, BN>(b, stream);
 }
 
@@ -555,6 +566,7 @@ cudaError_t grads(const FfnShape& s, const __nv_bfloat16* x, size_t x_stride, co
   if (out.dw_up) weight(out.dw_up, d_up, F, x, H, x_stride);
   if (out.dw_down) weight(out.dw_down, dy, H, h, F, F);
   if (out.dx && !input_first) input();
+  b.args.dependent = out.dx || out.dw_gate || out.dw_up;  // d_gate and d_up come from the launch before
   return launch<kPlain, BN>(b, stream);
 }
 
@@ -562,22 +574,39 @@ cudaError_t grads(const FfnShape& s, const __nv_bfloat16* x, size_t x_stride, co
 
 cudaError_t launch_ffn_gate_up(const FfnShape& s, const __nv_bfloat16* x, size_t x_stride, const __nv_bfloat16* gate,
                                const __nv_bfloat16* up, __nv_bfloat16* h, float* stored, cudaStream_t stream) {
-  return gate_up<256>(s, x, x_stride, gate, up, h, stored, stream);
+  return narrow_tiles(tiles_of(s.tokens, s.inter, 128), tiles_of(s.tokens, s.inter, 64))
+             ? gate_up<128>(s, x, x_stride, gate, up, h, stored, stream)
+             : gate_up<256>(s, x, x_stride, gate, up, h, stored, stream);
 }
 cudaError_t launch_ffn_down(const FfnShape& s, const __nv_bfloat16* h, const __nv_bfloat16* down, __nv_bfloat16* out,
                             cudaStream_t stream) {
-  return down_product<256>(s, h, down, out, stream);
+  return narrow_tiles(tiles_of(s.tokens, s.hidden, 256), tiles_of(s.tokens, s.hidden, 128))
+             ? down_product<128>(s, h, down, out, stream)
+             : down_product<256>(s, h, down, out, stream);
 }
 cudaError_t launch_ffn_d_gate_up(const FfnShape& s, const __nv_bfloat16* dy, const __nv_bfloat16* down,
                                  const float* stored, __nv_bfloat16* d_gate, __nv_bfloat16* d_up,
                                  cudaStream_t stream) {
-  return d_gate_up<256>(s, dy, down, stored, d_gate, d_up, stream);
+  return narrow_tiles(tiles_of(s.tokens, s.inter, 256), tiles_of(s.tokens, s.inter, 128))
+             ? d_gate_up<128>(s, dy, down, stored, d_gate, d_up, stream)
+             : d_gate_up<256>(s, dy, down, stored, d_gate, d_up, stream);
 }
 cudaError_t launch_ffn_grads(const FfnShape& s, const __nv_bfloat16* x, size_t x_stride, const __nv_bfloat16* gate,
                              const __nv_bfloat16* up, const __nv_bfloat16* h, const __nv_bfloat16* dy,
                              const __nv_bfloat16* d_gate, const __nv_bfloat16* d_up, const FfnGrads& out,
                              cudaStream_t stream) {
-  return grads<256>(s, x, x_stride, gate, up, h, dy, d_gate, d_up, out, stream);
+  // tiles of two lengths: weigh them by their K blocks, in units of the longer ones
+  auto rounds = [&](int tile_n) {
+    const double t_blocks = blocks_of(s.tokens), f_blocks = 2 * blocks_of(s.inter);
+    const double work = (out.dx ? tiles_of(s.tokens, s.hidden, tile_n) * f_blocks : 0.0) +
+                        t_blocks * ((out.dw_gate ? tiles_of(s.inter, s.hidden, tile_n) : 0) +
+                                    (out.dw_up ? tiles_of(s.inter, s.hidden, tile_n) : 0) +
+                                    (out.dw_down ? tiles_of(s.hidden, s.inter, tile_n) : 0));
+    return work / std::max(t_blocks, f_blocks);
+  };
+  return narrow_tiles(rounds(256), rounds(128))
+             ? grads<128>(s, x, x_stride, gate, up, h, dy, d_gate, d_up, out, stream)
+             : grads<256>(s, x, x_stride, gate, up, h, dy, d_gate, d_up, out, stream);
 }
 
 cudaError_t ffn_status(int* status, cudaStream_t stream) {

@@ -106,9 +106,6 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
-__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // kFmt 0: bf16 weights; 32, 64, 128: 4-bit weights with that group size. A K step is 128 bytes of a
 // row in two halves, of which a quad of lanes reads 4 x 16 bytes each.
 template <int kFmt>
@@ -670,21 +667,6 @@ __global__ void __launch_bounds__(256) weighted_rows_kernel(const float* rows, c
   v.x = *reinterpret_cast<uint32_t*>(&lo);
   v.y = *reinterpret_cast<uint32_t*>(&hi);
   *reinterpret_cast<uint2*>(out + t * hidden + h) = v;
-}
-
-template <class K, class... A>
-cudaError_t launch_kernel(K kernel, dim3 grid, int threads, size_t smem, bool dependent, cudaStream_t stream, A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = dependent ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <int kFmt>
