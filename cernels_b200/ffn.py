@@ -22,7 +22,8 @@ from .ops import _check
 _BF16 = torch.bfloat16
 
 
-def _rows_ok(x: torch.Tensor) -> bool:
+def rows_ok(x: torch.Tensor) -> bool:
+    """Whether the kernels can read the rows of x where they lie."""
     return x.stride(1) == 1 and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0))
 
 
@@ -39,7 +40,7 @@ def _validate(x, gate_proj, up_proj, down_proj) -> _lib.FfnShape:
     _check(gate_proj.shape == (F, H) and up_proj.shape == (F, H), "gate_proj and up_proj must be [F, H]")
     _check(down_proj.shape == (H, F), "down_proj must be [H, F]")
     _check(H > 0 and F > 0 and H % 8 == 0 and F % 8 == 0, "H and F must be multiples of 8")
-    _check(_rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least H) apart")
+    _check(rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least H) apart")
     return _lib.FfnShape(T, H, F)
 
 

@@ -83,12 +83,60 @@ def _family(cls_name: str, kernels: Callable):
     return apply
 
 
+def _linear_family(cls_name: str):
+    """Experts of the LINEAR layout, with a variant that decodes on 4-bit copies of the weights (made
+    here, once: apply it again after changing them) and prefills on the bf16 ones."""
+    plain = _family(cls_name, _linear_kernels)
+
+    def apply(model, variant: str):
+        from .registry import moe_experts_w4
+
+        if variant != "custom_w4":
+            for mod in model.modules():
+                if type(mod).__name__ == cls_name:
+                    moe_experts_w4.release(mod)
+            return plain(model, variant)
+        for mod in model.modules():
+            if type(mod).__name__ == cls_name:
+                moe_experts_w4.prepare(mod)
+        return swap_experts(model, cls_name, _linear_kernels()[0], moe_experts_w4.decode_kernel)
+
+    return apply
+
+
+def swap_mlps(model: torch.nn.Module, cls_name: str, custom: bool) -> int:
+    """Sets (or restores) the forward of every `cls_name` instance, a dense gated MLP (gate_proj, up_proj,
+    down_proj), to the gated feed-forward operator, which is differentiable. Returns the number of
+    modules touched; raises when the model has none."""
+    from .registry import gated_ffn
+
+    mods = [m for m in model.modules() if type(m).__name__ == cls_name]
+    if not mods:
+        raise RuntimeError(f"no {cls_name} modules found — wrong model for this swap")
+    for mod in mods:
+        if "forward" in vars(mod):
+            del mod.forward
+        if custom:
+            gated_ffn.check_module(mod)
+            mod.forward = lambda x, _m=mod: gated_ffn.kernel(x, _m)
+    return len(mods)
+
+
+def _mlp_family(cls_name: str):
+    return lambda model, variant: swap_mlps(model, cls_name, variant != "stock")
+
+
+_LINEAR_VARIANTS = ("stock", "custom_prefill", "custom", "custom_w4")
+
 SWAPS = {
     # the reference's two models (their experts classes need transformers >= 5.10)
-    "north_mini_code": (_family("Cohere2MoeExperts", _linear_kernels), ("stock", "custom_prefill", "custom")),
-    "deepseek_ocr_2": (_family("DeepseekOcr2TextExperts", _linear_kernels), ("stock", "custom_prefill", "custom")),
+    "north_mini_code": (_linear_family("Cohere2MoeExperts"), _LINEAR_VARIANTS),
+    "deepseek_ocr_2": (_linear_family("DeepseekOcr2TextExperts"), _LINEAR_VARIANTS),
     # experts classes of the installed transformers with the same contracts
-    "deepseek_v2": (_family("DeepseekV2Experts", _linear_kernels), ("stock", "custom_prefill", "custom")),
-    "qwen3_next": (_family("Qwen3NextExperts", _linear_kernels), ("stock", "custom_prefill", "custom")),
+    "deepseek_v2": (_linear_family("DeepseekV2Experts"), _LINEAR_VARIANTS),
+    "qwen3_next": (_linear_family("Qwen3NextExperts"), _LINEAR_VARIANTS),
     "gpt_oss": (_family("GptOssExperts", _gpt_oss_kernels), ("stock", "custom_prefill", "custom")),
+    # the dense layers and shared experts beside them, for training and serving
+    "deepseek_v2_mlp": (_mlp_family("DeepseekV2MLP"), ("stock", "custom")),
+    "qwen3_next_mlp": (_mlp_family("Qwen3NextMLP"), ("stock", "custom")),
 }

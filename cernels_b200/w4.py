@@ -18,7 +18,7 @@ import ctypes
 import torch
 
 from . import _lib
-from .ffn import _call, _rows_ok, _stride
+from .ffn import _call, rows_ok, _stride
 from .ops import DECODE_MAX_PAIRS, _check
 
 _BF16 = torch.bfloat16
@@ -65,7 +65,7 @@ def _linear_w4(x, qweight, scales):
     T, K = x.shape
     N = qweight.shape[0]
     group = _check_w4("qweight", qweight, scales, (N,), K, x.device)
-    _check(_rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least K) apart")
+    _check(rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least K) apart")
     out = x.new_empty((T, N))
     if T and N:
         _call(x.device, "cernels_linear_w4", T, N, K, group, x.data_ptr(), _stride(x), qweight.data_ptr(),
