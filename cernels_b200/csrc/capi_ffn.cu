@@ -46,7 +46,7 @@ size_t act_bytes(const cernels_ffn_shape* s) {
 bool few(const cernels_ffn_shape* s) { return s->tokens <= kSkinnyMaxColumns; }
 
 int balanced_columns(int tokens, int k, int group) {
-  const int most = skinny_columns(kSkinnyMaxColumns, k, group, 0);
+  const int most = skinny_columns(kSkinnyMaxColumns, k, group, 0, 0);
   if (most == 0) return 0;
   const int passes = (tokens + most - 1) / most;
   return (tokens + passes - 1) / passes;
@@ -67,7 +67,7 @@ int check_moe_w4(const cernels_moe_shape* s, int group) {
   const int rc = check_group(group, s->hidden, s->intermediate);
   if (rc) return rc;
   const int pairs = s->tokens * s->topk, longest = s->hidden > s->intermediate ? s->hidden : s->intermediate;
-  return skinny_columns(1, longest, group, pairs) ? CERNELS_OK : CERNELS_E_UNSUPPORTED;
+  return skinny_columns(1, longest, group, pairs, s->experts) ? CERNELS_OK : CERNELS_E_UNSUPPORTED;
 }
 
 struct MoeW4Workspace {
@@ -119,7 +119,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
   if (!aligned(out) || !aligned(workspace)) return CERNELS_E_ALIGNMENT;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const FfnShape s = shape_of(shape);
-  if (few(shape) && skinny_columns(1, s.hidden, 0, 0) && skinny_columns(1, s.inter, 0, 0)) {
+  if (few(shape) && skinny_columns(1, s.hidden, 0, 0, 0) && skinny_columns(1, s.inter, 0, 0, 0)) {
     SkinnyArgs a{};
     a.x = in(x);
     a.x_stride = static_cast<size_t>(x_stride);
@@ -279,7 +279,7 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   a.rows = shape->intermediate;
   // 4 columns are the cheapest tile; an expert with more pairs is read again for each 4 (or 8)
   const int want = a.pairs > 4 * a.experts ? 8 : 4;
-  a.cols = skinny_columns(want, a.k, group, a.pairs);
+  a.cols = skinny_columns(want, a.k, group, a.pairs, a.experts);
   cudaError_t err = launch_skinny(a, group, true, false, st);
   if (err != cudaSuccess) return code_of(err);
   a.x = ws.act;
@@ -295,7 +295,7 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   a.out_stride = H;
   a.k = shape->intermediate;
   a.rows = shape->hidden;
-  a.cols = skinny_columns(want, a.k, group, a.pairs);
+  a.cols = skinny_columns(want, a.k, group, a.pairs, a.experts);
   a.dependent = 1;
   err = launch_skinny(a, group, false, true, st);
   if (err == cudaSuccess)

@@ -85,9 +85,9 @@ struct SkinnyArgs {
   int dependent;              // x is written by the kernel launched just before on this stream
 };
 
-// Columns per tile for a reduction of `k` (group as below; pairs 0 without routing): at
+// Columns per tile for a reduction of `k` (group as below; pairs and experts 0 without routing): at
 // most `want`, kSkinnyMaxColumns and what shared memory holds of x. 0 when not even one row fits.
-int skinny_columns(int want, int k, int group, int pairs);
+int skinny_columns(int want, int k, int group, int pairs, int experts);
 // group: 0 for bf16 weights, 32 / 64 / 128 for 4 bits. gate_up: out = silu(w0 x) * (w1 x).
 cudaError_t launch_skinny(const SkinnyArgs& a, int group, bool gate_up, bool out_f32, cudaStream_t stream);
 cudaError_t launch_weighted_rows(const float* rows, const int32_t* indices, const float* weights, int tokens, int topk,

@@ -138,11 +138,12 @@ struct Item {
 __host__ __device__ constexpr int part_buffers(int warps) { return warps == 8 ? 2 : 1; }
 
 struct SkinnySmem {
-  size_t ring, part, units, x, items, ids, lead, rank, first, order, total;
+  size_t ring, part, units, x, items, ids, lead, count, first, rank, list, order, total;
 };
 
-// blocks: of 128 values in padded_k (0 for bf16); pairs: 0 without routing
-__host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int cols, int padded_k, int blocks, int pairs) {
+// blocks: of 128 values in padded_k (0 for bf16); pairs and experts: 0 without routing
+__host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int cols, int padded_k, int blocks, int pairs,
+                                                int experts) {
   SkinnySmem s;
   size_t off = 0;
   s.ring = off;
@@ -159,10 +160,14 @@ __host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int cols, 
   s.items = off;
   off += n * sizeof(Item);
   s.lead = off;
-  off += n * 4;
+  off += static_cast<size_t>(experts) * 4;
+  s.count = off;
+  off += static_cast<size_t>(experts) * 4;
+  s.first = off;
+  off += static_cast<size_t>(experts) * 4;
   s.rank = off;
   off += n * 2;
-  s.first = off;
+  s.list = off;
   off += n * 2;
   s.order = off;
   off += n * 2;
@@ -170,61 +175,55 @@ __host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int cols, 
   return s;
 }
 
-// Groups the (token, slot) pairs by expert, experts in order of first use and pairs in their own
-// order, into items of at most `cols` columns. Every CTA does this for itself, each pair by
-// comparing itself with all others (one warp walking through them took 4 us for 232 pairs). Returns the
-// number of items.
+// Groups the (token, slot) pairs by expert, experts in order of first use and pairs in their own order, into
+// items of at most `cols` columns. Every CTA does this for itself, and all come to the same lists: what
+// the counters' atomics leave open is put in order again by each pair looking through its expert's. (One
+// warp walking through all pairs took 4 us for 232 of them.) Returns the number of items.
 __device__ int build_items(const SkinnyArgs& a, uint8_t* smem, const SkinnySmem& lay) {
   int* ids = reinterpret_cast<int*>(smem + lay.ids);
   Item* items = reinterpret_cast<Item*>(smem + lay.items);
-  uint32_t* lead = reinterpret_cast<uint32_t*>(smem + lay.lead);  // an expert's first pair: items << 16 | pairs before it
+  int* count = reinterpret_cast<int*>(smem + lay.count);
+  int* first = reinterpret_cast<int*>(smem + lay.first);  // an expert's first pair
+  int* lead = reinterpret_cast<int*>(smem + lay.lead);    // and its first place in `order`
   uint16_t* rank = reinterpret_cast<uint16_t*>(smem + lay.rank);
-  uint16_t* first = reinterpret_cast<uint16_t*>(smem + lay.first);
+  uint16_t* list = reinterpret_cast<uint16_t*>(smem + lay.list);  // places as the atomics gave them out
   uint16_t* order = reinterpret_cast<uint16_t*>(smem + lay.order);
   int* n_items = reinterpret_cast<int*>(smem + lay.total - 16);
-  const int padded = (a.pairs + 3) / 4 * 4;
-  for (int p = threadIdx.x; p < padded; p += blockDim.x) {
-    const int e = p < a.pairs ? a.indices[p] : -1;
+  for (int p = threadIdx.x; p < a.pairs; p += blockDim.x) {
+    const int e = a.indices[p];
     ids[p] = e >= 0 && e < a.experts ? e : -1;
   }
-  __syncthreads();
-  for (int p = threadIdx.x; p < a.pairs; p += blockDim.x) {
-    const int e = ids[p];
-    int before = 0, all = 0, at = p;
-    for (int i = 0; i < padded; i += 4) {
-      const int4 v = *reinterpret_cast<const int4*>(ids + i);
-      const int other[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool same = other[j] == e;
-        all += same;
-        before += same && i + j < p;
-        if (same) at = min(at, i + j);
-      }
-    }
-    rank[p] = static_cast<uint16_t>(before);
-    first[p] = static_cast<uint16_t>(at);
-    lead[p] = e >= 0 && before == 0 ? static_cast<uint32_t>((all + a.cols - 1) / a.cols) << 16 | all : 0;
+  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+    count[e] = 0;
+    first[e] = a.pairs;
   }
+  __syncthreads();
+  for (int p = threadIdx.x; p < a.pairs; p += blockDim.x)
+    if (ids[p] >= 0) {
+      rank[p] = static_cast<uint16_t>(atomicAdd(&count[ids[p]], 1));
+      atomicMin(&first[ids[p]], p);
+    }
   __syncthreads();
   if (threadIdx.x < 32) {
     const int lane = threadIdx.x;
-    uint32_t total = 0;
+    uint32_t total = 0;  // items << 16 | places
     for (int p0 = 0; p0 < a.pairs; p0 += 32) {
       const int p = p0 + lane;
-      const uint32_t mine = p < a.pairs ? lead[p] : 0;
+      const int e = p < a.pairs ? ids[p] : -1;
+      const int n = e >= 0 && first[e] == p ? count[e] : 0;
+      const uint32_t mine = static_cast<uint32_t>((n + a.cols - 1) / a.cols) << 16 | static_cast<uint32_t>(n);
       uint32_t sum = mine;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
         const uint32_t v = __shfl_up_sync(0xffffffffu, sum, d);
         if (lane >= d) sum += v;
       }
-      const uint32_t start = total + sum - mine;
-      if (mine != 0) {
-        lead[p] = start;
-        const int n = mine & 0xffff, from = start & 0xffff;
+      if (n != 0) {
+        const uint32_t start = total + sum - mine;
+        const int from = start & 0xffff;
+        lead[e] = from;
         Item* to = items + (start >> 16);
-        for (int i = 0; i * a.cols < n; ++i) to[i] = Item{ids[p], from + i * a.cols, min(a.cols, n - i * a.cols)};
+        for (int i = 0; i * a.cols < n; ++i) to[i] = Item{e, from + i * a.cols, min(a.cols, n - i * a.cols)};
       }
       total += __shfl_sync(0xffffffffu, sum, 31);
     }
@@ -232,7 +231,16 @@ __device__ int build_items(const SkinnyArgs& a, uint8_t* smem, const SkinnySmem&
   }
   __syncthreads();
   for (int p = threadIdx.x; p < a.pairs; p += blockDim.x)
-    if (ids[p] >= 0) order[(lead[first[p]] & 0xffff) + rank[p]] = static_cast<uint16_t>(p);
+    if (ids[p] >= 0) list[lead[ids[p]] + rank[p]] = static_cast<uint16_t>(p);
+  __syncthreads();
+  for (int p = threadIdx.x; p < a.pairs; p += blockDim.x) {
+    const int e = ids[p];
+    if (e < 0) continue;
+    const int from = lead[e], n = count[e];
+    int before = 0;
+    for (int i = 0; i < n; ++i) before += list[from + i] < p;
+    order[from + before] = static_cast<uint16_t>(p);
+  }
   __syncthreads();
   return *n_items;
 }
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   const int x_bytes = x_row_bytes(padded_k);
   const bool routed = a.indices != nullptr;
   const SkinnySmem lay = carve_smem(kWarps, F::kSlot, a.cols, padded_k, kFmt == 0 ? 0 : padded_k / 128,
-                                    routed ? a.pairs : 0);
+                                    routed ? a.pairs : 0, routed ? a.experts : 0);
   float* part = reinterpret_cast<float*>(smem + lay.part);
   const int blocks = padded_k / 128;
   float* units_of_x = reinterpret_cast<float*>(smem + lay.units);  // [column][block]
@@ -286,60 +294,69 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   constexpr int kPerStep = kFmt == 0 ? 64 : 2 * F::kGroups;  // values (bf16) or groups
   int load_item = begin / per_item, load_unit = begin - load_item * per_item;  // position of the stream
   int load_left = (end - begin) * per_warp, load_step = kw;
-  const uint8_t *wa = nullptr, *wb = nullptr;
-  const uint16_t* sw = nullptr;  // scales of the row that this lane fetches them for, from a word's start
-  int s_odd = 0;                 // that row's scales start at the word's second half
-  uint32_t odd_a = 0, odd_b = 0;  // the same for the rows it computes, of the unit being consumed
+  // Eight lanes copy a row's 128 bytes of a step, four rows at once: whole lines, half the tag lookups of the
+  // lanes' own rows and quarters. Scales: lane (g, q) copies word q of rows g and g + 8.
+  const uint8_t *w_first = nullptr, *w_second = nullptr;  // rows lane / 8 of the tile's halves
+  int w_next_first = 0, w_next_second = 0;                // distance to rows lane / 8 + 4
+  const uint16_t *s_first = nullptr, *s_second = nullptr;  // scales of rows g, g + 8, from a word's start
+  int odd_first = 0, odd_second = 0;                       // they start at the word's second half
+  uint32_t odd_a = 0, odd_b = 0;  // the same, of the unit being consumed
+  const int piece = lane & 7;     // 16 bytes of the row: half piece / 4, quarter piece % 4
   auto point = [&] {
     const int e = routed ? items[load_item].expert : 0;
     const int base = (load_unit * tiles_at_once + rt) * kOut;
-    const int ra = min(base + g, a.rows - 1);
-    const int rb = kGateUp ? ra : min(base + g + 8, a.rows - 1);
-    const uint8_t* second = kGateUp ? a.w1 : a.w0;
-    const int at = kw * 128 + q * 16;
-    wa = a.w0 + static_cast<size_t>(e) * a.w_expert + static_cast<size_t>(ra) * row_bytes + at;
-    wb = second + static_cast<size_t>(e) * a.w_expert + static_cast<size_t>(rb) * row_bytes + at;
+    const int second = kGateUp ? 0 : 8;
+    auto row_of = [&](int r) { return static_cast<size_t>(min(base + r, a.rows - 1)); };
+    const int r = lane >> 3;
+    const uint8_t* from = a.w0 + static_cast<size_t>(e) * a.w_expert + kw * 128 + piece * 16;
+    const uint8_t* up = (kGateUp ? a.w1 : a.w0) + static_cast<size_t>(e) * a.w_expert + kw * 128 + piece * 16;
+    w_first = from + row_of(r) * row_bytes;
+    w_second = up + row_of(r + second) * row_bytes;
+    w_next_first = static_cast<int>((row_of(r + 4) - row_of(r)) * row_bytes);
+    w_next_second = static_cast<int>((row_of(r + second + 4) - row_of(r + second)) * row_bytes);
     if constexpr (kFmt != 0) {
-      const int r = lane & 15;
-      const int row = min(base + (kGateUp ? r & 7 : r), a.rows - 1);
-      const uint16_t* from = (kGateUp && r >= 8 ? a.s1 : a.s0) + static_cast<size_t>(e) * a.s_expert +
-                             static_cast<size_t>(row) * row_groups + kw * kPerStep;
-      s_odd = static_cast<int>(reinterpret_cast<uintptr_t>(from) >> 1 & 1);
-      sw = from - s_odd;
+      auto scales = [&](const uint16_t* s, size_t row, int& odd) {
+        s += static_cast<size_t>(e) * a.s_expert + row * row_groups + kw * kPerStep;
+        odd = static_cast<int>(reinterpret_cast<uintptr_t>(s) >> 1 & 1);
+        return s - odd;
+      };
+      s_first = scales(a.s0, row_of(g), odd_first);
+      s_second = scales(kGateUp ? a.s1 : a.s0, row_of(g + second), odd_second);
     }
   };
-  // Lane q copies bytes 16 q of its two rows' halves. `left`: groups (bf16: values) of the row from
-  // this step on.
   uint8_t* ring = smem + lay.ring + static_cast<size_t>(warp) * kDepth * F::kSlot;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-  auto copy_half = [&](uint32_t dst, const uint8_t* w, int h, bool whole, int left) {
-    const int first = kFmt == 0 ? h * 32 + q * 8 : h * F::kGroups + q * F::kGroups / 4;
-    copy_async<16>(dst, w + h * 64, whole || first < left ? 16 : 0);
-  };
   int load_slot = 0;
   auto issue = [&] {
     if (load_left != 0) {
       const int left = (kFmt == 0 ? a.k : row_groups) - load_step * kPerStep;
       const uint32_t at = ring_at + load_slot * F::kSlot;
-      const uint32_t dst = at + g * F::kRow + q * 16;
-      const bool whole = left >= kPerStep;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        copy_half(dst + h * F::kHalfBytes, wa, h, whole, left);
-        copy_half(dst + h * F::kHalfBytes + 8 * F::kRow, wb, h, whole, left);
-      }
-      wa += a.k_warps * 128;
-      wb += a.k_warps * 128;
+      const uint32_t dst = at + (piece >> 2) * F::kHalfBytes + (lane >> 3) * F::kRow + (piece & 3) * 16;
+      // first value (bf16) or group of this lane's 16 bytes
+      const int first = kFmt == 0 ? piece * 8 : (piece >> 2) * F::kGroups + (piece & 3) * F::kGroups / 4;
+      const int valid = left >= kPerStep || first < left ? 16 : 0;
+      copy_async<16>(dst, w_first, valid);
+      copy_async<16>(dst + 4 * F::kRow, w_first + w_next_first, valid);
+      copy_async<16>(dst + 8 * F::kRow, w_second, valid);
+      copy_async<16>(dst + 12 * F::kRow, w_second + w_next_second, valid);
+      w_first += a.k_warps * 128;
+      w_second += a.k_warps * 128;
       if constexpr (kFmt != 0) {
-        // two words of 16 rows at a time: this lane's row (lane % 16) and words lane / 16, + 2, ..
-        const uint32_t to = at + F::kScaleAt + lane * 4;
-        const int need = left > 0 ? min(left, 2 * F::kGroups) + s_odd : 0;  // scales from the word's start on
+        const uint32_t to = at + F::kScaleAt + g * 4;
+        auto copy_scales = [&](uint32_t to, const uint16_t* s, int odd) {
+          const int need = left > 0 ? min(left, 2 * F::kGroups) + odd : 0;  // scales from the word's start on
 #pragma unroll
-        for (int i = 0; i < (F::kScaleWords + 1) / 2; ++i) {
-          const int word = 2 * i + (lane >> 4);
-          if (word < F::kScaleWords) copy_async<4>(to + i * 128, sw + 2 * word, max(0, min(4, 2 * (need - 2 * word))));
-        }
-        sw += a.k_warps * kPerStep;
+          for (int i = 0; i < (F::kScaleWords + 3) / 4; ++i) {
+            const int word = 4 * i + q;
+            // the last word counts only where the row starts in the middle of the first
+            if (word < F::kScaleWords && (word < F::kScaleWords - 1 || odd))
+              copy_async<4>(to + word * 64, s + 2 * word, max(0, min(4, 2 * (need - 2 * word))));
+          }
+        };
+        copy_scales(to, s_first, odd_first);
+        copy_scales(to + 32, s_second, odd_second);
+        s_first += a.k_warps * kPerStep;
+        s_second += a.k_warps * kPerStep;
       }
       load_slot = load_slot + 1 == kDepth ? 0 : load_slot + 1;
       --load_left;
@@ -409,22 +426,23 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
           // 2^13 <= largest / 2^e < 2^14 (less for values whose unit, or its 16th, would be subnormal)
           const int unit_exp = max(static_cast<int>(top >> 23) - 13, 5);
           const float inverse = __uint_as_float(static_cast<uint32_t>(254 - unit_exp) << 23);
-          uint32_t hi[2] = {0, 0}, lo[2] = {0, 0};  // even and odd positions
+          uint32_t n[8];  // the nearest integer, in the low half of the float's bits
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const uint32_t bits = j & 1 ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16;
-            // the nearest integer in the low half of the float's bits, in two's complement
-            const uint32_t n = __float_as_uint(fmaf(__uint_as_float(bits), inverse, kFloatBiasValue));
-            hi[j & 1] |= (n + 128 >> 8 & 255u) << (8 * (j >> 1));
-            lo[j & 1] |= (n & 255u) << (8 * (j >> 1));
+            n[j] = __float_as_uint(fmaf(__uint_as_float(bits), inverse, kFloatBiasValue));
           }
+          auto bytes = [&](uint32_t selector, int odd, uint32_t add) {  // one byte of n[odd], n[odd + 2], ..
+            return __byte_perm(__byte_perm(n[odd] + add, n[odd + 2] + add, selector),
+                               __byte_perm(n[odd + 4] + add, n[odd + 6] + add, selector), 0x5410);
+          };
+          v[b] = make_uint4(bytes(0x51, 0, 128), bytes(0x51, 1, 128), bytes(0x40, 0, 0), bytes(0x40, 1, 0));
           if (k8 % 16 == 0)
             units_of_x[c * blocks + k8 / 16] =
                 __uint_as_float(top >= 0x7f800000u ? 0x7fc00000u : static_cast<uint32_t>(unit_exp - 4) << 23);
           constexpr unsigned kPer = kFmt / 8;  // pieces per group
           const unsigned in = k8 % kPer;
           at = k8 - in + (in % F::kWords) * 4 + in / F::kWords;  // group | quarter | word -> group | word | quarter
-          v[b] = make_uint4(hi[0], hi[1], lo[0], lo[1]);
         }
         *reinterpret_cast<uint4*>(xs + static_cast<size_t>(c) * x_bytes + at * 16) = v[b];
       }
@@ -674,7 +692,8 @@ size_t smem_bytes(const SkinnyArgs& a, int warps) {
   const int step = Format<kFmt>::kStep;
   const int padded = (a.k + step - 1) / step * step;
   const bool routed = a.indices != nullptr;
-  return carve_smem(warps, Format<kFmt>::kSlot, a.cols, padded, kFmt == 0 ? 0 : padded / 128, routed ? a.pairs : 0)
+  return carve_smem(warps, Format<kFmt>::kSlot, a.cols, padded, kFmt == 0 ? 0 : padded / 128, routed ? a.pairs : 0,
+                    routed ? a.experts : 0)
       .total;
 }
 
@@ -703,7 +722,7 @@ cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   const int items = routed ? a.pairs : (a.tokens + a.cols - 1) / a.cols;
   const int slots = device_sm_count() * (kWarps == 8 && 2 * (smem + 1024) <= kSmemPerSm ? 2 : 1);
-  // Warps to a tile: a unit costs its steps per warp and about 1.5 more for the barrier and the additions at
+  // Warps to a tile: a unit costs its steps per warp and about one more for the barrier and the additions at
   // its end, and the CTA with the most units decides. (On 16384 x 8192 at 7 columns 2 warps take 24.4 us and
   // 16 take 29.0.) With routing the expected number of experts stands for the items.
   const double likely = routed ? a.experts * (1.0 - std::exp(-static_cast<double>(a.pairs) / a.experts)) : 0.0;
@@ -712,7 +731,7 @@ cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
   for (int k = 1; k <= kWarps; k *= 2) {
     const int rows = (kGateUp ? 8 : 16) * (kWarps / k);
     const long long n = expected * ((a.rows + rows - 1) / rows);
-    const long long cost = (n + slots - 1) / slots * (2 * ((steps + k - 1) / k) + 3);
+    const long long cost = (n + slots - 1) / slots * (2 * ((steps + k - 1) / k) + 2);
     if (best == 0 || cost < best) {
       best = cost;
       a.k_warps = k;
@@ -745,12 +764,12 @@ cudaError_t launch_format(const SkinnyArgs& a, int group, cudaStream_t stream) {
 
 }  // namespace
 
-int skinny_columns(int want, int k, int group, int pairs) {
+int skinny_columns(int want, int k, int group, int pairs, int experts) {
   const int step = group == 0 ? Format<0>::kStep : Format<32>::kStep;
   const int slot = group == 0 ? Format<0>::kSlot : group == 128 ? Format<128>::kSlot : group == 64 ? Format<64>::kSlot : Format<32>::kSlot;
   const int padded = (k + step - 1) / step * step;
   int cols = want < kSkinnyMaxColumns ? want : kSkinnyMaxColumns;
-  while (cols > 0 && carve_smem(8, slot, cols, padded, group == 0 ? 0 : padded / 128, pairs).total > kMaxSmem)
+  while (cols > 0 && carve_smem(8, slot, cols, padded, group == 0 ? 0 : padded / 128, pairs, experts).total > kMaxSmem)
     --cols;
   return cols;
 }
