@@ -29,6 +29,7 @@
 #include "ffn_internal.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace cernels {
 namespace {
@@ -92,6 +93,13 @@ __device__ __forceinline__ Two fma(Two a, Two b, Two c) {
 
 // Copies `bytes` (4, 8 or 16) to shared memory without a register; reads only the first `valid` of
 // them (0: none) and fills the rest with zeros.
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(kBytes) : "memory");
+}
 template <int kBytes>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, int valid) {
   if constexpr (kBytes == 16)
@@ -318,7 +326,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
       auto scales = [&](const uint16_t* s, size_t row, int& odd) {
         s += static_cast<size_t>(e) * a.s_expert + row * row_groups + kw * kPerStep;
         odd = static_cast<int>(reinterpret_cast<uintptr_t>(s) >> 1 & 1);
-        return s - odd;
+        return s - odd + 2 * q;  // this lane's first word
       };
       s_first = scales(a.s0, row_of(g), odd_first);
       s_second = scales(kGateUp ? a.s1 : a.s0, row_of(g + second), odd_second);
@@ -326,39 +334,58 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   };
   uint8_t* ring = smem + lay.ring + static_cast<size_t>(warp) * kDepth * F::kSlot;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-  int load_slot = 0;
+  uint32_t load_at = ring_at;  // slot that the next step goes to
+  const uint32_t lane_at = (piece >> 2) * F::kHalfBytes + (lane >> 3) * F::kRow + (piece & 3) * 16;
+  const uint32_t scale_at = F::kScaleAt + g * 4 + q * 64;
+  const int step_bytes = a.k_warps * 128, step_scales = a.k_warps * kPerStep;
+  // A row's words of scales beyond the first four (lane q has word q), and its last one, which counts only
+  // where the row starts in the middle of the first.
+  auto copy_step = [&](auto whole, int left) {
+    // first value (bf16) or group of this lane's 16 bytes
+    const int first = kFmt == 0 ? piece * 8 : (piece >> 2) * F::kGroups + (piece & 3) * F::kGroups / 4;
+    auto row = [&](uint32_t to, const uint8_t* from) {
+      if constexpr (whole.value)
+        copy_async<16>(load_at + lane_at + to, from);
+      else
+        copy_async<16>(load_at + lane_at + to, from, first < left ? 16 : 0);
+    };
+    row(0, w_first);
+    row(4 * F::kRow, w_first + w_next_first);
+    row(8 * F::kRow, w_second);
+    row(12 * F::kRow, w_second + w_next_second);
+    if constexpr (kFmt != 0) {
+      auto scales = [&](uint32_t to, const uint16_t* from, int odd) {
+        const int need = left > 0 ? min(left, kPerStep) + odd : 0;  // from the word's start on
+#pragma unroll
+        for (int i = 0; i < (F::kScaleWords + 3) / 4; ++i) {
+          const int word = 4 * i + q;
+          if (word < F::kScaleWords && (word < F::kScaleWords - 1 || odd)) {
+            if constexpr (whole.value)
+              copy_async<4>(load_at + scale_at + to + i * 256, from + 8 * i);
+            else
+              copy_async<4>(load_at + scale_at + to + i * 256, from + 8 * i, max(0, min(4, 2 * (need - 2 * word))));
+          }
+        }
+      };
+      scales(0, s_first, odd_first);
+      scales(32, s_second, odd_second);
+    }
+  };
   auto issue = [&] {
     if (load_left != 0) {
       const int left = (kFmt == 0 ? a.k : row_groups) - load_step * kPerStep;
-      const uint32_t at = ring_at + load_slot * F::kSlot;
-      const uint32_t dst = at + (piece >> 2) * F::kHalfBytes + (lane >> 3) * F::kRow + (piece & 3) * 16;
-      // first value (bf16) or group of this lane's 16 bytes
-      const int first = kFmt == 0 ? piece * 8 : (piece >> 2) * F::kGroups + (piece & 3) * F::kGroups / 4;
-      const int valid = left >= kPerStep || first < left ? 16 : 0;
-      copy_async<16>(dst, w_first, valid);
-      copy_async<16>(dst + 4 * F::kRow, w_first + w_next_first, valid);
-      copy_async<16>(dst + 8 * F::kRow, w_second, valid);
-      copy_async<16>(dst + 12 * F::kRow, w_second + w_next_second, valid);
-      w_first += a.k_warps * 128;
-      w_second += a.k_warps * 128;
+      if (left > kPerStep)  // more of the row follows: nothing to cut off, not even half of the last word
+        copy_step(std::true_type{}, left);
+      else
+        copy_step(std::false_type{}, left);
+      w_first += step_bytes;
+      w_second += step_bytes;
       if constexpr (kFmt != 0) {
-        const uint32_t to = at + F::kScaleAt + g * 4;
-        auto copy_scales = [&](uint32_t to, const uint16_t* s, int odd) {
-          const int need = left > 0 ? min(left, 2 * F::kGroups) + odd : 0;  // scales from the word's start on
-#pragma unroll
-          for (int i = 0; i < (F::kScaleWords + 3) / 4; ++i) {
-            const int word = 4 * i + q;
-            // the last word counts only where the row starts in the middle of the first
-            if (word < F::kScaleWords && (word < F::kScaleWords - 1 || odd))
-              copy_async<4>(to + word * 64, s + 2 * word, max(0, min(4, 2 * (need - 2 * word))));
-          }
-        };
-        copy_scales(to, s_first, odd_first);
-        copy_scales(to + 32, s_second, odd_second);
-        s_first += a.k_warps * kPerStep;
-        s_second += a.k_warps * kPerStep;
+        s_first += step_scales;
+        s_second += step_scales;
       }
-      load_slot = load_slot + 1 == kDepth ? 0 : load_slot + 1;
+      load_at += F::kSlot;
+      if (load_at == ring_at + kDepth * F::kSlot) load_at = ring_at;
       --load_left;
       load_step += a.k_warps;
       if (load_step - kw == per_warp * a.k_warps) {
@@ -478,7 +505,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
 
-  int units_left = end - begin, i = 0, buffer = 0, slot = 0;
+  int units_left = end - begin, i = 0, buffer = 0;
+  const uint8_t* at = ring;  // slot of the step being consumed
   auto point_scales = [&] {
     if constexpr (kFmt != 0) {
       const int base = (unit * tiles_at_once + rt) * kOut;
@@ -496,7 +524,6 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     wait_copies<kDepth - 1>();
     __syncwarp();  // the scales were fetched by other lanes
     if (step < steps) {
-      const uint8_t* at = ring + slot * F::kSlot;
       const uint8_t* x_at[NT];
 #pragma unroll
       for (int n = 0; n < NT; ++n) x_at[n] = xcol[n] + step * (F::kStep * 2);
@@ -606,7 +633,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     }
     __syncwarp();  // every lane has read the slot
     issue();
-    slot = slot + 1 == kDepth ? 0 : slot + 1;
+    at += F::kSlot;
+    if (at == ring + kDepth * F::kSlot) at = ring;
     if (++i == per_warp) {
       // ---- end of the unit: add the sums of each tile's warps (in warp order) and write
       i = 0;
