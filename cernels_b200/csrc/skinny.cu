@@ -146,7 +146,7 @@ struct Item {
 __host__ __device__ constexpr int part_buffers(int warps) { return warps == 8 ? 2 : 1; }
 
 struct SkinnySmem {
-  size_t ring, part, units, x, items, ids, lead, count, first, rank, list, order, total;
+  size_t ring, part, units, x, items, ids, lead, count, first, sums, rank, list, order, total;
 };
 
 // blocks: of 128 values in padded_k (0 for bf16); pairs and experts: 0 without routing
@@ -173,6 +173,8 @@ __host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int cols, 
   off += static_cast<size_t>(experts) * 4;
   s.first = off;
   off += static_cast<size_t>(experts) * 4;
+  s.sums = off;
+  off += (n + 31) / 32 * 4;
   s.rank = off;
   off += n * 2;
   s.list = off;
@@ -212,30 +214,37 @@ __device__ int build_items(const SkinnyArgs& a, uint8_t* smem, const SkinnySmem&
       atomicMin(&first[ids[p]], p);
     }
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const int lane = threadIdx.x;
-    uint32_t total = 0;  // items << 16 | places
-    for (int p0 = 0; p0 < a.pairs; p0 += 32) {
-      const int p = p0 + lane;
-      const int e = p < a.pairs ? ids[p] : -1;
-      const int n = e >= 0 && first[e] == p ? count[e] : 0;
-      const uint32_t mine = static_cast<uint32_t>((n + a.cols - 1) / a.cols) << 16 | static_cast<uint32_t>(n);
-      uint32_t sum = mine;
+  // places and items before each expert: within 32 pairs, then over all of them
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  uint32_t* sums = reinterpret_cast<uint32_t*>(smem + lay.sums);  // items << 16 | places, of 32 pairs each
+  for (int chunk = threadIdx.x >> 5; chunk * 32 < a.pairs; chunk += warps) {
+    const int p = chunk * 32 + lane;
+    const int e = p < a.pairs ? ids[p] : -1;
+    const int n = e >= 0 && first[e] == p ? count[e] : 0;
+    const uint32_t mine = static_cast<uint32_t>((n + a.cols - 1) / a.cols) << 16 | static_cast<uint32_t>(n);
+    uint32_t sum = mine;
 #pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t v = __shfl_up_sync(0xffffffffu, sum, d);
-        if (lane >= d) sum += v;
-      }
-      if (n != 0) {
-        const uint32_t start = total + sum - mine;
-        const int from = start & 0xffff;
-        lead[e] = from;
-        Item* to = items + (start >> 16);
-        for (int i = 0; i * a.cols < n; ++i) to[i] = Item{e, from + i * a.cols, min(a.cols, n - i * a.cols)};
-      }
-      total += __shfl_sync(0xffffffffu, sum, 31);
+    for (int d = 1; d < 32; d <<= 1) {
+      const uint32_t v = __shfl_up_sync(0xffffffffu, sum, d);
+      if (lane >= d) sum += v;
     }
-    if (lane == 0) *n_items = total >> 16;
+    if (n != 0) lead[e] = static_cast<int>(sum - mine);
+    if (lane == 31) sums[chunk] = sum;
+  }
+  __syncthreads();
+  for (int chunk = threadIdx.x >> 5; chunk * 32 < a.pairs; chunk += warps) {
+    const int p = chunk * 32 + lane;
+    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < chunk ? sums[lane] : 0);
+    const int e = p < a.pairs ? ids[p] : -1;
+    const int n = e >= 0 && first[e] == p ? count[e] : 0;
+    if (n != 0) {
+      const uint32_t start = before + static_cast<uint32_t>(lead[e]);
+      const int from = start & 0xffff;
+      lead[e] = from;
+      Item* to = items + (start >> 16);
+      for (int i = 0; i * a.cols < n; ++i) to[i] = Item{e, from + i * a.cols, min(a.cols, n - i * a.cols)};
+    }
+    if ((chunk + 1) * 32 >= a.pairs && lane == 0) *n_items = before + sums[chunk] >> 16;
   }
   __syncthreads();
   for (int p = threadIdx.x; p < a.pairs; p += blockDim.x)
@@ -399,85 +408,115 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     }
     commit_copies();
   };
-  point();
-#pragma unroll
-  for (int d = 0; d < kDepth; ++d) issue();
-  if (a.dependent) wait_for_previous_kernel();  // x is the previous kernel's output
-
   // ---- x rows of an item, 8 values (a piece) at a time, in the order in which the weights lie
-  auto load_x = [&](const Item& it) {
-    const unsigned pieces = static_cast<unsigned>(padded_k) / 8;  // 4 bits: a multiple of 32, so a warp stays within a row
-    const unsigned total = it.count * pieces;
-    if constexpr (kFmt == 0) {
-      const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(xs));
-      for (unsigned i = threadIdx.x; i < total; i += kThreads) {
-        const unsigned c = i / pieces, k8 = i - c * pieces;
-        const size_t row = it.first + c;
-        copy_async<16>(to + c * x_bytes + k8 * 16, a.x + row * a.x_stride + k8 * 8, static_cast<int>(k8) * 8 < a.k ? 16 : 0);
-      }
-      commit_copies();
-      wait_copies<0>();
-      return;
-    }
-    constexpr int kBatch = 8;  // loads on their way at once
-    for (unsigned i0 = threadIdx.x; i0 < total; i0 += kThreads * kBatch) {
-      uint4 v[kBatch];
+  // 4 bits: a warp takes a row's 256 values at once (a chunk), kBatch chunks on their way together.
+  constexpr int kBatch = 8;
+  const unsigned inverse_steps = (1u << 20) / steps + 1;  // chunk / steps, exact for the up to 16 * 128 chunks
+  auto fetch_x = [&](const Item& it, int first_chunk, uint4 (&v)[kBatch]) {
 #pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const unsigned i = i0 + b * kThreads;
-        v[b] = make_uint4(0, 0, 0, 0);
-        if (i < total) {
-          const unsigned c = i / pieces, k8 = i - c * pieces;
-          int row = it.first + static_cast<int>(c);
-          if (routed) {
-            row = order[row];
-            if (!a.x_by_pair) row /= a.topk;
-          }
-          if (static_cast<int>(k8) * 8 < a.k)
-            v[b] = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(row) * a.x_stride + k8 * 8);
+    for (int b = 0; b < kBatch; ++b) {
+      const unsigned chunk = first_chunk + b * kWarps;
+      v[b] = make_uint4(0, 0, 0, 0);
+      if (static_cast<int>(chunk) < it.count * steps) {
+        const int c = static_cast<int>(chunk * inverse_steps >> 20);
+        const int k = (static_cast<int>(chunk) - c * steps) * F::kStep + lane * 8;
+        int row = it.first + c;
+        if (routed) {
+          row = order[row];
+          if (!a.x_by_pair) row /= a.topk;
         }
-      }
-#pragma unroll
-      for (int b = 0; b < kBatch; ++b) {
-        const unsigned i = i0 + b * kThreads;
-        if (i >= total) break;  // whole warps, where lanes work together
-        const unsigned c = i / pieces, k8 = i - c * pieces;
-        unsigned at = k8;
-        if constexpr (kFmt != 0) {
-          const uint32_t words[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
-          uint32_t top = 0;  // largest magnitude, as bits
-#pragma unroll
-          for (int j = 0; j < 4; ++j) top = max(top, max(words[j] << 16 & 0x7fff0000u, words[j] & 0x7fff0000u));
-#pragma unroll
-          for (unsigned d = 8; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-          // 2^13 <= largest / 2^e < 2^14 (less for values whose unit, or its 16th, would be subnormal)
-          const int unit_exp = max(static_cast<int>(top >> 23) - 13, 5);
-          const float inverse = __uint_as_float(static_cast<uint32_t>(254 - unit_exp) << 23);
-          uint32_t n[8];  // the nearest integer, in the low half of the float's bits
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const uint32_t bits = j & 1 ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16;
-            n[j] = __float_as_uint(fmaf(__uint_as_float(bits), inverse, kFloatBiasValue));
-          }
-          auto bytes = [&](uint32_t selector, int odd, uint32_t add) {  // one byte of n[odd], n[odd + 2], ..
-            return __byte_perm(__byte_perm(n[odd] + add, n[odd + 2] + add, selector),
-                               __byte_perm(n[odd + 4] + add, n[odd + 6] + add, selector), 0x5410);
-          };
-          v[b] = make_uint4(bytes(0x51, 0, 128), bytes(0x51, 1, 128), bytes(0x40, 0, 0), bytes(0x40, 1, 0));
-          if (k8 % 16 == 0)
-            units_of_x[c * blocks + k8 / 16] =
-                __uint_as_float(top >= 0x7f800000u ? 0x7fc00000u : static_cast<uint32_t>(unit_exp - 4) << 23);
-          constexpr unsigned kPer = kFmt / 8;  // pieces per group
-          const unsigned in = k8 % kPer;
-          at = k8 - in + (in % F::kWords) * 4 + in / F::kWords;  // group | quarter | word -> group | word | quarter
-        }
-        *reinterpret_cast<uint4*>(xs + static_cast<size_t>(c) * x_bytes + at * 16) = v[b];
+        if (k < a.k) v[b] = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(row) * a.x_stride + k);
       }
     }
   };
+  auto store_x = [&](const Item& it, int first_chunk, const uint4 (&v)[kBatch]) {
+    if constexpr (kFmt != 0) {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const unsigned chunk = first_chunk + b * kWarps;
+        if (static_cast<int>(chunk) >= it.count * steps) break;
+        const int c = static_cast<int>(chunk * inverse_steps >> 20);
+        const unsigned k8 = (chunk - c * steps) * (F::kStep / 8) + lane;
+        const uint32_t words[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
+        uint32_t top = 0;  // the block's largest magnitude, as bits
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, max(words[j] << 16 & 0x7fff0000u, words[j] & 0x7fff0000u));
+#pragma unroll
+        for (unsigned d = 8; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+        // 2^13 <= largest / 2^e < 2^14 (less for values whose unit, or its 16th, would be subnormal)
+        const int unit_exp = max(static_cast<int>(top >> 23) - 13, 5);
+        const float inverse = __uint_as_float(static_cast<uint32_t>(254 - unit_exp) << 23);
+        uint32_t n[8];  // the nearest integer, in the low half of the float's bits
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const uint32_t bits = j & 1 ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16;
+          n[j] = __float_as_uint(fmaf(__uint_as_float(bits), inverse, kFloatBiasValue));
+        }
+        auto bytes = [&](uint32_t selector, int odd, uint32_t add) {  // one byte of n[odd], n[odd + 2], ..
+          return __byte_perm(__byte_perm(n[odd] + add, n[odd + 2] + add, selector),
+                             __byte_perm(n[odd + 4] + add, n[odd + 6] + add, selector), 0x5410);
+        };
+        if (k8 % 16 == 0)
+          units_of_x[c * blocks + k8 / 16] =
+              __uint_as_float(top >= 0x7f800000u ? 0x7fc00000u : static_cast<uint32_t>(unit_exp - 4) << 23);
+        constexpr unsigned kPer = kFmt / 8;  // pieces per group
+        const unsigned in = k8 % kPer;
+        // group | lane of the quad | word  ->  group | word | lane
+        const unsigned at = k8 - in + (in % F::kWords) * 4 + in / F::kWords;
+        *reinterpret_cast<uint4*>(xs + static_cast<size_t>(c) * x_bytes + at * 16) =
+            make_uint4(bytes(0x51, 0, 128), bytes(0x51, 1, 128), bytes(0x40, 0, 0), bytes(0x40, 1, 0));
+      }
+    }
+  };
+  auto copy_x = [&](const Item& it) {  // bf16
+    const unsigned pieces = static_cast<unsigned>(padded_k) / 8;
+    const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(xs));
+    for (unsigned i = threadIdx.x; i < it.count * pieces; i += kThreads) {
+      const unsigned c = i / pieces, k8 = i - c * pieces;
+      const size_t row = it.first + c;
+      copy_async<16>(to + c * x_bytes + k8 * 16, a.x + row * a.x_stride + k8 * 8, static_cast<int>(k8) * 8 < a.k ? 16 : 0);
+    }
+    commit_copies();
+  };
+  auto load_x = [&](const Item& it, int first_chunk) {
+    if constexpr (kFmt == 0) {
+      copy_x(it);
+      wait_copies<0>();
+    } else {
+      for (int chunk = first_chunk; chunk < it.count * steps; chunk += kWarps * kBatch) {
+        uint4 v[kBatch];
+        fetch_x(it, chunk, v);
+        store_x(it, chunk, v);
+      }
+    }
+  };
+
+  // x before the weights where it is there already: its first loads then do not queue behind them
   int item_index = begin / per_item, unit = begin - item_index * per_item;
   Item item = item_of(item_index);
-  load_x(item);
+  uint4 first_x[kBatch];
+  if (!a.dependent) {
+    if constexpr (kFmt == 0)
+      copy_x(item);
+    else
+      fetch_x(item, warp, first_x);
+  }
+  point();
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) issue();
+  if (a.dependent) {
+    wait_for_previous_kernel();  // x is its output
+    if constexpr (kFmt != 0)
+      fetch_x(item, warp, first_x);
+    else
+      load_x(item, 0);
+  } else if constexpr (kFmt == 0) {
+    wait_copies<kDepth>();
+  }
+  if constexpr (kFmt != 0) {
+    store_x(item, warp, first_x);
+    load_x(item, warp + kWarps * kBatch);
+  }
   __syncthreads();
   // Columns past the item's last read its last one again: their sums are never used.
   const uint8_t* xcol[NT];
@@ -680,7 +719,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
       if (++unit == per_item) {  // the next item's x rows; every warp has used the old ones
         unit = 0;
         item = item_of(++item_index);
-        load_x(item);
+        load_x(item, warp);
         __syncthreads();
         point_x();
       }
@@ -750,16 +789,17 @@ cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   const int items = routed ? a.pairs : (a.tokens + a.cols - 1) / a.cols;
   const int slots = device_sm_count() * (kWarps == 8 && 2 * (smem + 1024) <= kSmemPerSm ? 2 : 1);
-  // Warps to a tile: a unit costs its steps per warp and about one more for the barrier and the additions at
-  // its end, and the CTA with the most units decides. (On 16384 x 8192 at 7 columns 2 warps take 24.4 us and
-  // 16 take 29.0.) With routing the expected number of experts stands for the items.
+  // Warps to a tile: a unit costs its steps per warp and about 1.5 more for the barrier and the additions at
+  // its end, and the CTA with the most units decides. (On 16384 x 8192 at 7
+  // columns 2 warps take 24.4 us and 16 take 29.0.) With routing the expected number of experts stands for
+  // the items.
   const double likely = routed ? a.experts * (1.0 - std::exp(-static_cast<double>(a.pairs) / a.experts)) : 0.0;
   const long long expected = routed ? static_cast<long long>(likely) + 1 : items;
   long long best = 0;
   for (int k = 1; k <= kWarps; k *= 2) {
     const int rows = (kGateUp ? 8 : 16) * (kWarps / k);
     const long long n = expected * ((a.rows + rows - 1) / rows);
-    const long long cost = (n + slots - 1) / slots * (2 * ((steps + k - 1) / k) + 2);
+    const long long cost = (n + slots - 1) / slots * (2 * ((steps + k - 1) / k) + 3);
     if (best == 0 || cost < best) {
       best = cost;
       a.k_warps = k;
