@@ -41,9 +41,14 @@ size_t act_bytes(const cernels_ffn_shape* s) {
   return align_up(static_cast<size_t>(s->tokens) * s->intermediate * 2, 256);
 }
 
-// A few tokens: the weights' bytes bound the work, and the kernel that streams them reads them at the
-// same rate for 1 to 16 rows.
-bool few(const cernels_ffn_shape* s) { return s->tokens <= kSkinnyMaxColumns; }
+// A few tokens: the weights' bytes bound the work. The kernel that streams them reads them once per 16 tokens,
+// up to 48 from L2 where they fit half of it; the tile kernel takes a full tile's time for any number. (us,
+// streamed and tiled: H = F = 2880, 50 MB: 18.0 at 16 tokens, 24.5 and 30.3 at 48, 36.0 and 30.3 at 64; H = 4096,
+// F = 8192, 201 MB: 54.4 at 16, 64.8 and 62.8 at 24.)
+bool few(const cernels_ffn_shape* s) {
+  const long long weights = 6ll * s->hidden * s->intermediate;
+  return s->tokens <= kSkinnyMaxColumns || (s->tokens <= 48 && weights <= (64ll << 20));
+}
 
 int balanced_columns(int tokens, int k, int group) {
   const int most = skinny_columns(kSkinnyMaxColumns, k, group, 0, 0);
