@@ -37,6 +37,7 @@ namespace {
 constexpr int kMaxSmem = 232448;        // per CTA
 constexpr int kSmemPerSm = 228 * 1024;  // 1 KB of it is taken per CTA
 constexpr int kDepth = 3;  // steps in flight per warp
+constexpr int kParts = 2;  // 64-byte parts of a row in a step: whole lines (4, at depth 2, measured the same)
 constexpr int kCtas = 2;   // per SM; fewer where x rows need the shared memory
 
 __device__ __forceinline__ float sigmoid(float g) { return __fdividef(1.0f, 1.0f + __expf(-g)); }
@@ -114,21 +115,21 @@ __device__ __forceinline__ void wait_copies() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
 }
 
-// kFmt 0: bf16 weights; 32, 64, 128: 4-bit weights with that group size. A K step is 128 bytes of a
-// row in two halves, of which a quad of lanes reads 4 x 16 bytes each.
+// kFmt 0: bf16 weights; 32, 64, 128: 4-bit weights with that group size. A K step is kParts parts of 64 bytes
+// of a row, of which a quad of lanes reads 16 bytes each.
 template <int kFmt>
 struct Format {
-  static constexpr int kHalf = kFmt == 0 ? 32 : 128;
-  static constexpr int kStep = 2 * kHalf;
-  static constexpr int kGroups = kFmt == 0 ? 1 : 128 / kFmt;  // per half
+  static constexpr int kPart = kFmt == 0 ? 32 : 128;  // values
+  static constexpr int kStep = kParts * kPart;
+  static constexpr int kGroups = kFmt == 0 ? 1 : 128 / kFmt;  // per part
   static constexpr int kWords = kFmt == 0 ? 1 : kFmt / 32;    // 8-code words per lane and group
-  // A warp's ring slot: a step's 16 rows, [half][row][64 bytes], and the words that hold the rows'
-  // 2 kGroups scales, [word][row]; rows may start in the middle of a word. An mma takes the same
-  // group from all lanes, 4 kWords bytes each: rows lie so far apart that those reads meet no bank twice.
-  static constexpr int kRow = kFmt == 64 ? 96 : kFmt == 32 ? 80 : 64;
-  static constexpr int kHalfBytes = 16 * kRow;
-  static constexpr int kScaleWords = kFmt == 0 ? 0 : kGroups + 1;
-  static constexpr int kScaleAt = 2 * kHalfBytes;
+  // A warp's ring slot: a step's 16 rows, [part][row][64 bytes], and the words that hold the rows' scales, [word][row];
+  // rows may start in the middle of a word. Where an mma takes the same group from all lanes (4 kWords bytes
+  // each), a row's 16-byte pieces are exchanged so that those reads meet no bank twice: piece ^ swizzle(row).
+  static constexpr int kPartBytes = 16 * 64;
+  static constexpr int kScaleWords = kFmt == 0 ? 0 : kParts * kGroups / 2 + 1;
+  static constexpr int kScaleAt = kParts * kPartBytes;
+  __device__ static int swizzle(int row) { return kFmt == 32 ? row >> 1 & 3 : kFmt == 64 ? row & 2 : 0; }
   static constexpr int kSlot = kScaleAt + kScaleWords * 64;
 };
 
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   // ---- weights: this lane's two rows of a unit, and the stream of steps through them
   const size_t row_bytes = kFmt == 0 ? static_cast<size_t>(a.k) * 2 : static_cast<size_t>(a.k) / 2;
   const int row_groups = kFmt == 0 ? 0 : a.k / (kFmt == 0 ? 1 : kFmt);
-  constexpr int kPerStep = kFmt == 0 ? 64 : 2 * F::kGroups;  // values (bf16) or groups
+  constexpr int kPerStep = kFmt == 0 ? F::kStep : kParts * F::kGroups;  // values (bf16) or groups
   int load_item = begin / per_item, load_unit = begin - load_item * per_item;  // position of the stream
   int load_left = (end - begin) * per_warp, load_step = kw;
   // Eight lanes copy a row's 128 bytes of a step, four rows at once: whole lines, half the tag lookups of the
@@ -318,15 +319,15 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   const uint16_t *s_first = nullptr, *s_second = nullptr;  // scales of rows g, g + 8, from a word's start
   int odd_first = 0, odd_second = 0;                       // they start at the word's second half
   uint32_t odd_a = 0, odd_b = 0;  // the same, of the unit being consumed
-  const int piece = lane & 7;     // 16 bytes of the row: half piece / 4, quarter piece % 4
+  const int piece = lane & 7;     // 16 bytes of the 128: part piece / 4, lane of the quad piece % 4
   auto point = [&] {
     const int e = routed ? items[load_item].expert : 0;
     const int base = (load_unit * tiles_at_once + rt) * kOut;
     const int second = kGateUp ? 0 : 8;
     auto row_of = [&](int r) { return static_cast<size_t>(min(base + r, a.rows - 1)); };
     const int r = lane >> 3;
-    const uint8_t* from = a.w0 + static_cast<size_t>(e) * a.w_expert + kw * 128 + piece * 16;
-    const uint8_t* up = (kGateUp ? a.w1 : a.w0) + static_cast<size_t>(e) * a.w_expert + kw * 128 + piece * 16;
+    const uint8_t* from = a.w0 + static_cast<size_t>(e) * a.w_expert + kw * (kParts * 64) + piece * 16;
+    const uint8_t* up = (kGateUp ? a.w1 : a.w0) + static_cast<size_t>(e) * a.w_expert + kw * (kParts * 64) + piece * 16;
     w_first = from + row_of(r) * row_bytes;
     w_second = up + row_of(r + second) * row_bytes;
     w_next_first = static_cast<int>((row_of(r + 4) - row_of(r)) * row_bytes);
@@ -344,24 +345,30 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   uint8_t* ring = smem + lay.ring + static_cast<size_t>(warp) * kDepth * F::kSlot;
   const uint32_t ring_at = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
   uint32_t load_at = ring_at;  // slot that the next step goes to
-  const uint32_t lane_at = (piece >> 2) * F::kHalfBytes + (lane >> 3) * F::kRow + (piece & 3) * 16;
+  // rows r and r + 8 share a swizzle, rows r and r + 4 (r < 4) do not
+  auto piece_at = [&](int row) { return (piece >> 2) * F::kPartBytes + row * 64 + ((piece & 3) ^ F::swizzle(row)) * 16; };
+  const uint32_t lane_at = piece_at(lane >> 3), next_at = piece_at((lane >> 3) + 4);
   const uint32_t scale_at = F::kScaleAt + g * 4 + q * 64;
-  const int step_bytes = a.k_warps * 128, step_scales = a.k_warps * kPerStep;
+  const int step_bytes = a.k_warps * (kParts * 64), step_scales = a.k_warps * kPerStep;
   // A row's words of scales beyond the first four (lane q has word q), and its last one, which counts only
   // where the row starts in the middle of the first.
   auto copy_step = [&](auto whole, int left) {
-    // first value (bf16) or group of this lane's 16 bytes
-    const int first = kFmt == 0 ? piece * 8 : (piece >> 2) * F::kGroups + (piece & 3) * F::kGroups / 4;
-    auto row = [&](uint32_t to, const uint8_t* from) {
-      if constexpr (whole.value)
-        copy_async<16>(load_at + lane_at + to, from);
-      else
-        copy_async<16>(load_at + lane_at + to, from, first < left ? 16 : 0);
-    };
-    row(0, w_first);
-    row(4 * F::kRow, w_first + w_next_first);
-    row(8 * F::kRow, w_second);
-    row(12 * F::kRow, w_second + w_next_second);
+#pragma unroll
+    for (int c = 0; c < kParts / 2; ++c) {
+      // first value (bf16) or group of this lane's 16 bytes
+      const int first = kFmt == 0 ? c * 64 + piece * 8 : (2 * c + (piece >> 2)) * F::kGroups + (piece & 3) * F::kGroups / 4;
+      auto row = [&](uint32_t to, const uint8_t* from) {
+        to += load_at + 2 * c * F::kPartBytes;
+        if constexpr (whole.value)
+          copy_async<16>(to, from + c * 128);
+        else
+          copy_async<16>(to, from + c * 128, first < left ? 16 : 0);
+      };
+      row(lane_at, w_first);
+      row(next_at, w_first + w_next_first);
+      row(lane_at + 8 * 64, w_second);
+      row(next_at + 8 * 64, w_second + w_next_second);
+    }
     if constexpr (kFmt != 0) {
       auto scales = [&](uint32_t to, const uint16_t* from, int odd) {
         const int need = left > 0 ? min(left, kPerStep) + odd : 0;  // from the word's start on
@@ -411,15 +418,16 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   // ---- x rows of an item, 8 values (a piece) at a time, in the order in which the weights lie
   // 4 bits: a warp takes a row's 256 values at once (a chunk), kBatch chunks on their way together.
   constexpr int kBatch = 8;
-  const unsigned inverse_steps = (1u << 20) / steps + 1;  // chunk / steps, exact for the up to 16 * 128 chunks
+  const int row_chunks = padded_k / 256;
+  const unsigned inverse_chunks = (1u << 20) / (row_chunks ? row_chunks : 1) + 1;  // chunk / row_chunks, exact for up to 16 * 128
   auto fetch_x = [&](const Item& it, int first_chunk, uint4 (&v)[kBatch]) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const unsigned chunk = first_chunk + b * kWarps;
       v[b] = make_uint4(0, 0, 0, 0);
-      if (static_cast<int>(chunk) < it.count * steps) {
-        const int c = static_cast<int>(chunk * inverse_steps >> 20);
-        const int k = (static_cast<int>(chunk) - c * steps) * F::kStep + lane * 8;
+      if (static_cast<int>(chunk) < it.count * row_chunks) {
+        const int c = static_cast<int>(chunk * inverse_chunks >> 20);
+        const int k = (static_cast<int>(chunk) - c * row_chunks) * 256 + lane * 8;
         int row = it.first + c;
         if (routed) {
           row = order[row];
@@ -434,9 +442,9 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const unsigned chunk = first_chunk + b * kWarps;
-        if (static_cast<int>(chunk) >= it.count * steps) break;
-        const int c = static_cast<int>(chunk * inverse_steps >> 20);
-        const unsigned k8 = (chunk - c * steps) * (F::kStep / 8) + lane;
+        if (static_cast<int>(chunk) >= it.count * row_chunks) break;
+        const int c = static_cast<int>(chunk * inverse_chunks >> 20);
+        const unsigned k8 = (chunk - c * row_chunks) * 32 + lane;
         const uint32_t words[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
         uint32_t top = 0;  // the block's largest magnitude, as bits
 #pragma unroll
@@ -483,7 +491,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
       copy_x(it);
       wait_copies<0>();
     } else {
-      for (int chunk = first_chunk; chunk < it.count * steps; chunk += kWarps * kBatch) {
+      for (int chunk = first_chunk; chunk < it.count * row_chunks; chunk += kWarps * kBatch) {
         uint4 v[kBatch];
         fetch_x(it, chunk, v);
         store_x(it, chunk, v);
@@ -544,6 +552,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n][i] = 0.f;
 
+  const int swizzle = F::swizzle(g);  // of rows g and g + 8
   int units_left = end - begin, i = 0, buffer = 0;
   const uint8_t* at = ring;  // slot of the step being consumed
   auto point_scales = [&] {
@@ -573,14 +582,14 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
         sb[j] = *reinterpret_cast<const uint32_t*>(at + F::kScaleAt + j * 64 + 32 + g * 4);
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint8_t* ra = at + h * F::kHalfBytes + g * F::kRow;
-        const uint8_t* rb = ra + 8 * F::kRow;
+      for (int h = 0; h < kParts; ++h) {
+        const uint8_t* ra = at + h * F::kPartBytes + g * 64;
+        const uint8_t* rb = ra + 8 * 64;
         if constexpr (kFmt == 0) {
           const uint4 u = *reinterpret_cast<const uint4*>(ra + q * 16), v = *reinterpret_cast<const uint4*>(rb + q * 16);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const uint4 x4 = *reinterpret_cast<const uint4*>(x_at[n] + h * (F::kHalf * 2));
+            const uint4 x4 = *reinterpret_cast<const uint4*>(x_at[n] + h * (F::kPart * 2));
             mma_bf16(acc[n], u.x, v.x, u.y, v.y, x4.x, x4.y);
             mma_bf16(acc[n], u.z, v.z, u.w, v.w, x4.z, x4.w);
           }
@@ -593,19 +602,19 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
           } else if constexpr (kFmt == 64) {
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-              const uint2 u = *reinterpret_cast<const uint2*>(ra + s * 32 + q * 8);
-              const uint2 v = *reinterpret_cast<const uint2*>(rb + s * 32 + q * 8);
+              const uint2 u = *reinterpret_cast<const uint2*>(ra + ((2 * s + (q >> 1)) ^ swizzle) * 16 + (q & 1) * 8);
+              const uint2 v = *reinterpret_cast<const uint2*>(rb + ((2 * s + (q >> 1)) ^ swizzle) * 16 + (q & 1) * 8);
               aw[2 * s] = u.x, aw[2 * s + 1] = u.y;
               bw[2 * s] = v.x, bw[2 * s + 1] = v.y;
             }
           } else {
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-              aw[s] = *reinterpret_cast<const uint32_t*>(ra + s * 16 + q * 4);
-              bw[s] = *reinterpret_cast<const uint32_t*>(rb + s * 16 + q * 4);
+              aw[s] = *reinterpret_cast<const uint32_t*>(ra + (s ^ swizzle) * 16 + q * 4);
+              bw[s] = *reinterpret_cast<const uint32_t*>(rb + (s ^ swizzle) * 16 + q * 4);
             }
           }
-          // scale of group s of this half, of a row whose first is the low or (odd) the high half of word 0
+          // scale of group s of this part, of a row whose first is the low or (odd) the high half of word 0
           auto scale_of = [&](const uint32_t* words, uint32_t odd, int s) {
             const int gi = h * F::kGroups + s;
             const uint32_t v = __funnelshift_r(words[gi >> 1], words[(gi >> 1) + 1], odd * 16);
@@ -626,7 +635,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
               const uint32_t a2 = (u & 0xf0f0f0f0u) ^ 0x80808080u, a3 = (v & 0xf0f0f0f0u) ^ 0x80808080u;
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                const uint8_t* from = x_at[n] + h * (F::kHalf * 2) + (s * F::kWords + w) * 64;
+                const uint8_t* from = x_at[n] + h * (F::kPart * 2) + (s * F::kWords + w) * 64;
                 if constexpr (kPacked) {
                   const uint2 x2 = *reinterpret_cast<const uint2*>(from);
                   mma_bytes(high[n], w == 0 ? start : high[n], a0, a1, a2, a3, x2.x, x2.y);
@@ -652,7 +661,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
               }
             }
           }
-          const int block = step * 2 + h;
+          const int block = step * kParts + h;
           if constexpr (kPacked) {
             const float unit = units_at[0][0][block];
             acc[0][0] = fmaf(unit, block_p[0], acc[0][0]);
