@@ -136,7 +136,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
     a.rows = s.inter;
     a.tokens = s.tokens;
     a.cols = balanced_columns(s.tokens, s.hidden, 0);
-    cudaError_t e = launch_skinny(a, 0, true, false, st);
+    cudaError_t e = launch_skinny(a, 0, true, st);
     a.x = in(workspace);
     a.x_stride = static_cast<size_t>(s.inter);
     a.w0 = bytes(down_proj);
@@ -147,7 +147,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
     a.rows = s.hidden;
     a.cols = balanced_columns(s.tokens, s.inter, 0);
     a.dependent = 1;
-    if (e == cudaSuccess) e = launch_skinny(a, 0, false, false, st);
+    if (e == cudaSuccess) e = launch_skinny(a, 0, false, st);
     return code_of(e);
   }
   cudaError_t err = launch_ffn_gate_up(s, in(x), static_cast<size_t>(x_stride), in(gate_proj), in(up_proj),
@@ -236,7 +236,7 @@ int cernels_linear_w4(int32_t tokens, int32_t out_features, int32_t in_features,
   if (units > 0x7fffffffll) return CERNELS_E_UNSUPPORTED;
   rc = check_sm100();
   if (rc) return rc;
-  return code_of(launch_skinny(a, group, false, false, static_cast<cudaStream_t>(stream)));
+  return code_of(launch_skinny(a, group, false, static_cast<cudaStream_t>(stream)));
 }
 
 int cernels_moe_w4_workspace_bytes(const cernels_moe_shape* shape, int32_t group, size_t* bytes) {
@@ -285,7 +285,7 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   // 4 columns are the cheapest tile; an expert with more pairs is read again for each 4 (or 8)
   const int want = a.pairs > 4 * a.experts ? 8 : 4;
   a.cols = skinny_columns(want, a.k, group, a.pairs, a.experts);
-  cudaError_t err = launch_skinny(a, group, true, false, st);
+  cudaError_t err = launch_skinny(a, group, true, st);
   if (err != cudaSuccess) return code_of(err);
   a.x = ws.act;
   a.x_stride = F;
@@ -302,7 +302,8 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   a.rows = shape->hidden;
   a.cols = skinny_columns(want, a.k, group, a.pairs, a.experts);
   a.dependent = 1;
-  err = launch_skinny(a, group, false, true, st);
+  a.out_f32 = 1;
+  err = launch_skinny(a, group, false, st);
   if (err == cudaSuccess)
     err = launch_weighted_rows(ws.rows, indices, weights, shape->tokens, shape->topk, shape->experts, shape->hidden,
                                outp(out), st);

@@ -75,6 +75,7 @@ struct SkinnyArgs {
   size_t s_expert;            // scales between experts
   void* out;                  // bf16 or fp32 [column, rows], out_stride elements apart
   size_t out_stride;
+  int out_f32;
   int k, rows;                // reduction length; outputs per column (gate/up: F)
   int cols;                   // columns that a tile takes at once (skinny_columns())
   int tokens;                 // columns without routing
@@ -89,7 +90,7 @@ struct SkinnyArgs {
 // most `want`, kSkinnyMaxColumns and what shared memory holds of x. 0 when not even one row fits.
 int skinny_columns(int want, int k, int group, int pairs, int experts);
 // group: 0 for bf16 weights, 32 / 64 / 128 for 4 bits. gate_up: out = silu(w0 x) * (w1 x).
-cudaError_t launch_skinny(const SkinnyArgs& a, int group, bool gate_up, bool out_f32, cudaStream_t stream);
+cudaError_t launch_skinny(const SkinnyArgs& a, int group, bool gate_up, cudaStream_t stream);
 cudaError_t launch_weighted_rows(const float* rows, const int32_t* indices, const float* weights, int tokens, int topk,
                                  int experts, int hidden, __nv_bfloat16* out, cudaStream_t stream);
 

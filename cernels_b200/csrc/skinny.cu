@@ -8,8 +8,10 @@
 // 8 / KW tiles at once, KW warps to a tile: these take the tile's K steps in turn, so that
 // neighbouring warps read neighbouring bytes, and their sums are added in shared memory in warp order. A
 // CTA walks through a contiguous range of tiles with its x rows in shared memory and, per warp, the
-// weights of the next kDepth steps already on their way into registers, across tile borders:
-// up to 128 KB of weights in flight per SM.
+// weights of the next kDepth steps on their way into a ring of its own (cp.async, across tile borders): up to
+// 96 KB of weights in flight per SM. bf16 weights reach 5.5 of the measured 6.5 TB/s (one row of x, 201 MB in
+// 36.6 us). The same ring in registers gave 2.7 TB/s, and a third as much with 4-bit weights: a warp has too
+// few load counters to wait for one step and not for those behind it.
 //
 // mma.sync does the products: rows of W are the A operand, x columns the B operand. The order of k
 // within the reduction is free as long as A and B agree, so W is used as it lies in memory and x is
@@ -23,9 +25,11 @@
 // two mma's (up to 4 columns: two columns of one mma). This keeps 14 bits below the block's largest value, where
 // bf16 x holds 8 bits of each value: every x within 2^-6 of the largest is exact, the others are rounded by at
 // most 2^-14 of it, far below the rounding of the output. The sums of 16 (q - 8) hi and 16 (q - 8) lo over a
-// group are exact integers of at most 128 * 128 * 128 < 2^22, and they start at the integer whose bits are the float 1.5 * 2^23, so that their own
-// bits are that float plus the sum. From there on it is 32-bit floating arithmetic: scales are never
-// rounded and multiply each group's sum. A block of x that holds an infinity or a NaN makes its row NaN.
+// group are exact integers of at most 128 * 128 * 128 < 2^22, and they start at the integer whose bits are the
+// float 1.5 * 2^23, so that their own bits are that float plus the sum. From there on it is 32-bit floating
+// arithmetic: scales are never rounded and multiply each group's sum. A block of x that holds an infinity or
+// a NaN makes its row NaN. What bounds it now is instructions, 180 for 16 x 128 weights in groups of 32: experts
+// at 8 tokens take 87 us, without the copies 80, without the products 68, against 45 for their bytes.
 #include "ffn_internal.h"
 
 #include <cmath>
@@ -36,7 +40,7 @@ namespace {
 
 constexpr int kMaxSmem = 232448;        // per CTA
 constexpr int kSmemPerSm = 228 * 1024;  // 1 KB of it is taken per CTA
-constexpr int kDepth = 3;  // steps in flight per warp
+constexpr int kDepth = 3;  // steps in flight per warp; 4 measured the same where as many CTAs fit
 constexpr int kParts = 2;  // 64-byte parts of a row in a step: whole lines (4, at depth 2, measured the same)
 constexpr int kCtas = 2;   // per SM; fewer where x rows need the shared memory
 
@@ -263,7 +267,7 @@ __device__ int build_items(const SkinnyArgs& a, uint8_t* smem, const SkinnySmem&
   return *n_items;
 }
 
-template <int kFmt, bool kGateUp, int kCols, bool kOutF32, int kWarps>
+template <int kFmt, bool kGateUp, int kCols, int kWarps>
 __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_kernel(const SkinnyArgs a) {
   using F = Format<kFmt>;
   constexpr int kThreads = 32 * kWarps;
@@ -715,7 +719,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
         }
         if constexpr (kGateUp) v = v * sigmoid(v) * u;
         const size_t at = static_cast<size_t>(routed ? order[item.first + c] : item.first + c) * a.out_stride + row;
-        if constexpr (kOutF32)
+        if (a.out_f32)
           static_cast<float*>(a.out)[at] = v;
         else
           static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(v);
@@ -773,20 +777,20 @@ size_t smem_bytes(const SkinnyArgs& a, int warps) {
       .total;
 }
 
-template <int kFmt, bool kGateUp, int kCols, bool kOutF32, int kWarps>
+template <int kFmt, bool kGateUp, int kCols, int kWarps>
 cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream);
 
 // Eight warps a CTA and two CTAs an SM; where x rows leave room for one, sixteen warps if they fit.
-template <int kFmt, bool kGateUp, int kCols, bool kOutF32>
+template <int kFmt, bool kGateUp, int kCols>
 cudaError_t launch_tile(const SkinnyArgs& a, cudaStream_t stream) {
   const size_t two = smem_bytes<kFmt>(a, 8), one = smem_bytes<kFmt>(a, 16);
-  return 2 * (two + 1024) > kSmemPerSm && one <= kMaxSmem ? launch_warps<kFmt, kGateUp, kCols, kOutF32, 16>(a, stream)
-                                                          : launch_warps<kFmt, kGateUp, kCols, kOutF32, 8>(a, stream);
+  return 2 * (two + 1024) > kSmemPerSm && one <= kMaxSmem ? launch_warps<kFmt, kGateUp, kCols, 16>(a, stream)
+                                                          : launch_warps<kFmt, kGateUp, kCols, 8>(a, stream);
 }
 
-template <int kFmt, bool kGateUp, int kCols, bool kOutF32, int kWarps>
+template <int kFmt, bool kGateUp, int kCols, int kWarps>
 cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
-  const auto kernel = skinny_kernel<kFmt, kGateUp, kCols, kOutF32, kWarps>;
+  const auto kernel = skinny_kernel<kFmt, kGateUp, kCols, kWarps>;
   const int step = Format<kFmt>::kStep;
   const int steps = (a.k + step - 1) / step;
   const bool routed = a.indices != nullptr;
@@ -820,21 +824,22 @@ cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
   return launch_kernel(kernel, dim3(grid), 32 * kWarps, smem, a.dependent != 0, stream, a);
 }
 
-template <int kFmt, bool kGateUp, bool kOutF32>
+template <int kFmt, bool kGateUp>
 cudaError_t launch_columns(const SkinnyArgs& a, cudaStream_t stream) {
   if constexpr (kFmt != 0)
-    if (a.cols <= 4) return launch_tile<kFmt, kGateUp, 4, kOutF32>(a, stream);
-  return a.cols <= 8 ? launch_tile<kFmt, kGateUp, 8, kOutF32>(a, stream)
-                     : launch_tile<kFmt, kGateUp, 16, kOutF32>(a, stream);
+    if (a.cols <= 4) return launch_tile<kFmt, kGateUp, 4>(a, stream);
+  if (a.cols <= 8) return launch_tile<kFmt, kGateUp, 8>(a, stream);
+  if constexpr (kFmt == 0 || !kGateUp) return launch_tile<kFmt, kGateUp, 16>(a, stream);
+  return cudaErrorInvalidValue;  // 4-bit gate/up products are the experts', at most 8 columns
 }
 
-template <bool kGateUp, bool kOutF32>
+template <bool kGateUp>
 cudaError_t launch_format(const SkinnyArgs& a, int group, cudaStream_t stream) {
   switch (group) {
-    case 0: return launch_columns<0, kGateUp, kOutF32>(a, stream);
-    case 32: return launch_columns<32, kGateUp, kOutF32>(a, stream);
-    case 64: return launch_columns<64, kGateUp, kOutF32>(a, stream);
-    case 128: return launch_columns<128, kGateUp, kOutF32>(a, stream);
+    case 0: return launch_columns<0, kGateUp>(a, stream);
+    case 32: return launch_columns<32, kGateUp>(a, stream);
+    case 64: return launch_columns<64, kGateUp>(a, stream);
+    case 128: return launch_columns<128, kGateUp>(a, stream);
   }
   return cudaErrorInvalidValue;
 }
@@ -851,10 +856,9 @@ int skinny_columns(int want, int k, int group, int pairs, int experts) {
   return cols;
 }
 
-cudaError_t launch_skinny(const SkinnyArgs& a, int group, bool gate_up, bool out_f32, cudaStream_t stream) {
+cudaError_t launch_skinny(const SkinnyArgs& a, int group, bool gate_up, cudaStream_t stream) {
   if (a.cols < 1 || a.cols > kSkinnyMaxColumns) return cudaErrorInvalidValue;
-  if (gate_up) return out_f32 ? cudaErrorInvalidValue : launch_format<true, false>(a, group, stream);
-  return out_f32 ? launch_format<false, true>(a, group, stream) : launch_format<false, false>(a, group, stream);
+  return gate_up ? launch_format<true>(a, group, stream) : launch_format<false>(a, group, stream);
 }
 
 cudaError_t launch_weighted_rows(const float* rows, const int32_t* indices, const float* weights, int tokens, int topk,

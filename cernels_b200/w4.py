@@ -66,6 +66,8 @@ def _linear_w4(x, qweight, scales):
     N = qweight.shape[0]
     group = _check_w4("qweight", qweight, scales, (N,), K, x.device)
     _check(rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least K) apart")
+    if scales.data_ptr() % 4:  # rows of a slice may start in the middle of the words that the kernel copies
+        scales = scales.clone()
     out = x.new_empty((T, N))
     if T and N:
         _call(x.device, "cernels_linear_w4", T, N, K, group, x.data_ptr(), _stride(x), qweight.data_ptr(),

@@ -108,6 +108,28 @@ def test_gradients_against_differences():
 
 
 @gpu
+def test_more_than_2_31_stored_values():
+    """So many tokens that what the backward pass stores is indexed past 32 bits; the last rows' results
+    and input gradients, and weight gradients that only they feed."""
+    T, H, F = 131_200, 64, 8192
+    assert T * 2 * F > 2 ** 31
+    x, wg, wu, wd, _ = R.case(T, H, F, seed=14)
+    dy = torch.zeros(T, H, dtype=torch.bfloat16, device="cuda")
+    tail = slice(T - 40, T)
+    dy[tail] = R.case(40, H, 8, seed=15)[4]
+    t = leaves((x, wg, wu, wd))
+    y = cernels_b200.gated_ffn(*t)
+    got = torch.autograd.grad(y, t, dy)
+    want, bound, state = R.forward(x[tail], wg, wu, wd)
+    R.assert_within("y", y.detach()[tail], want, bound)
+    grads = R.backward(state, dy[tail])
+    R.assert_within("dx", got[0][tail], *grads[0])
+    assert not got[0][:T - 40].any()
+    for g, (w, b) in zip(got[1:], grads[1:]):  # the other rows add products of zeros
+        R.assert_within("dw", g, w, b)
+
+
+@gpu
 @pytest.mark.parametrize("T", [3, 70])
 @pytest.mark.parametrize("need", [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (1, 0, 0, 1), (0, 1, 1, 1)])
 def test_partial_gradients_are_the_same(T, need):

@@ -149,6 +149,8 @@ def test_linear_row_strides_empty_and_repeats():
     y = cernels_b200.linear_w4(x, q, s)
     assert torch.equal(y, cernels_b200.linear_w4(wide[::2, 16:144], q, s))
     assert torch.equal(y, cernels_b200.linear_w4(x, q, s))
+    q3, s3 = R.codes((24, 128), 128, 2)  # one scale a row: the slice's start is 2 bytes off a word
+    assert torch.equal(cernels_b200.linear_w4(x, q3[5:], s3[5:]), cernels_b200.linear_w4(x, q3, s3)[:, 5:])
     assert cernels_b200.linear_w4(x[:0], q, s).shape == (0, 24)
     assert cernels_b200.linear_w4(x, q[:0], s[:0]).shape == (5, 0)
 
@@ -242,6 +244,26 @@ def test_experts_wide_rows():
     x, w = rows(T, H, 7), experts(E, H, F, 64, 8)
     idx, p = routing(T, k, E, 9)
     assert_within("y", cernels_b200.moe_experts_decode_w4(x, *w, idx, p, k), *R.experts(x, *w, idx, p))
+
+
+@gpu
+def test_experts_beyond_32_bit_offsets():
+    """The last of so many experts that its codes start 2^31 bytes and more into the tensor."""
+    T, H, E, F = 2, 4096, 70, 8192
+    assert (E - 1) * 2 * F * (H // 2) > 2 ** 31
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    q1 = torch.zeros(E, 2 * F, H // 2, dtype=torch.uint8, device="cuda")
+    q2 = torch.zeros(E, H, F // 2, dtype=torch.uint8, device="cuda")
+    s1 = torch.zeros(E, 2 * F, H // 128, dtype=torch.bfloat16, device="cuda")
+    s2 = torch.zeros(E, H, F // 128, dtype=torch.bfloat16, device="cuda")
+    last = experts(1, H, F, 128, 3)
+    for t, v in zip((q1, s1, q2, s2), last):
+        t[E - 1] = v[0]
+    x = rows(T, H, 4)
+    idx = torch.full((T, 1), E - 1, dtype=torch.int32, device="cuda")
+    p = torch.rand(T, 1, generator=gen, device="cuda")
+    want, bound = R.experts(x, *last, torch.zeros_like(idx), p)
+    assert_within("y", cernels_b200.moe_experts_decode_w4(x, q1, s1, q2, s2, idx, p, 1), want, bound)
 
 
 @gpu
