@@ -146,7 +146,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
     a.k = s.inter;
     a.rows = s.hidden;
     a.cols = balanced_columns(s.tokens, s.inter, 0);
-    a.dependent = 1;
+    a.x_from_previous = 1;
     if (e == cudaSuccess) e = launch_skinny(a, 0, false, st);
     return code_of(e);
   }
@@ -301,7 +301,7 @@ int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group,
   a.k = shape->intermediate;
   a.rows = shape->hidden;
   a.cols = skinny_columns(want, a.k, group, a.pairs, a.experts);
-  a.dependent = 1;
+  a.x_from_previous = 1;
   a.out_f32 = 1;
   err = launch_skinny(a, group, false, st);
   if (err == cudaSuccess)

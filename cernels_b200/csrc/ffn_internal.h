@@ -7,14 +7,16 @@
 namespace cernels {
 
 #ifdef __CUDACC__
-// Programmatic dependent launch: a kernel launched as the dependent of the one before it on its
-// stream may start while that one runs, and waits here for its end before it touches its results. Every
-// CTA of a dependent kernel waits, so that its own end implies the other's.
-__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void let_next_kernel_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// Programmatic dependent launch: every kernel here may start while the one before it on its stream, whichever that
+// is, still runs, and waits for its end before it reads or writes what that one might write or read. All CTAs
+// wait, so that a kernel's end implies the ends of all before it; and only then do they let the next kernel
+// start, so that what a kernel reads before its own wait can be in the hands of its predecessor alone.
+__device__ __forceinline__ void wait_for_previous_kernel() {
+  asm volatile("griddepcontrol.wait;\n\tgriddepcontrol.launch_dependents;" ::: "memory");
+}
 
 template <class K, class... A>
-cudaError_t launch_kernel(K kernel, dim3 grid, int threads, size_t smem, bool dependent, cudaStream_t stream, A... args) {
+cudaError_t launch_kernel(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t stream, A... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -24,7 +26,7 @@ cudaError_t launch_kernel(K kernel, dim3 grid, int threads, size_t smem, bool de
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
-  cfg.numAttrs = dependent ? 1 : 0;
+  cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 #endif
@@ -83,7 +85,7 @@ struct SkinnyArgs {
   int pairs, topk, experts;
   int x_by_pair;              // x rows belong to pairs (else to tokens, pair / topk)
   int k_warps;                // warps that share a tile (the launcher sets it)
-  int dependent;              // x is written by the kernel launched just before on this stream
+  int x_from_previous;        // x is written by the kernel launched just before, which writes nothing else read here
 };
 
 // Columns per tile for a reduction of `k` (group as below; pairs and experts 0 without routing): at

@@ -78,7 +78,6 @@ struct PairArgs {
   float* gate_up;  // stored products (kGateUp writes when not null, kGradGateUp reads)
   int inter;       // F
   int row_blocks;  // ceil(T / 32)
-  int dependent;   // operands are written by the kernel launched just before on this stream
   unsigned long long wait_ns;
 };
 
@@ -150,7 +149,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  let_next_kernel_start();
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = pair_rank();
@@ -179,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   pair_sync();  // both CTAs' barriers exist before any remote arrive
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  if (args.dependent) wait_for_previous_kernel();
+  wait_for_previous_kernel();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA loads
@@ -473,8 +471,7 @@ cudaError_t launch(Builder& b, cudaStream_t stream) {
   const int pairs = b.args.total_tiles < max_pairs ? b.args.total_tiles : max_pairs;
   if (pairs <= 0) return cudaSuccess;
   b.args.wait_ns = wait_limit_ns(kWaitLimitNs);
-  return launch_kernel(pair_gemm_kernel<kEpi, BN>, dim3(2 * pairs), kThreads, C::kSmem, b.args.dependent != 0, stream, b.maps,
-                       b.args);
+  return launch_kernel(pair_gemm_kernel<kEpi, BN>, dim3(2 * pairs), kThreads, C::kSmem, stream, b.maps, b.args);
 }
 
 int tiles_of(int m, int n, int tile_n) { return (m + 2 * kBM - 1) / (2 * kBM) * ((n + tile_n - 1) / tile_n); }
@@ -513,7 +510,6 @@ cudaError_t down_product(const FfnShape& s, const __nv_bfloat16* h, const __nv_b
   p.a_map[0] = b.k_major(h, s.tokens, s.inter, s.inter, kBM);
   p.b_map[0] = b.k_major(down, s.hidden, s.inter, s.inter, BN / 2);
   p.out_map[0] = b.output(out, s.tokens, s.hidden);
-  b.args.dependent = 1;
   return launch<kPlain, BN>(b, stream);
 }
 
@@ -566,7 +562,6 @@ cudaError_t grads(const FfnShape& s, const __nv_bfloat16* x, size_t x_stride, co
   if (out.dw_up) weight(out.dw_up, d_up, F, x, H, x_stride);
   if (out.dw_down) weight(out.dw_down, dy, H, h, F, F);
   if (out.dx && !input_first) input();
-  b.args.dependent = out.dx || out.dw_gate || out.dw_up;  // d_gate and d_up come from the launch before
   return launch<kPlain, BN>(b, stream);
 }
 

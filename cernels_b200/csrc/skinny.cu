@@ -277,7 +277,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   static_assert(!kPacked || kFmt != 0, "bf16 x has no halves");
   constexpr int kOut = kGateUp ? 8 : 16;  // outputs per tile and column
   extern __shared__ __align__(16) uint8_t smem[];
-  let_next_kernel_start();
+  if (!a.x_from_previous) wait_for_previous_kernel();  // it may have written anything read here
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, q = lane & 3;  // mma row (and x column) of this lane, its quarter of a half step
   const int kw = warp % a.k_warps, rt = warp / a.k_warps;
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   const int begin = static_cast<int>(units * blockIdx.x / gridDim.x);
   const int end = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x);
   if (begin >= end) {
-    if (a.dependent) wait_for_previous_kernel();  // this kernel never ends before the one it follows
+    if (a.x_from_previous) wait_for_previous_kernel();
     return;
   }
 
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   int item_index = begin / per_item, unit = begin - item_index * per_item;
   Item item = item_of(item_index);
   uint4 first_x[kBatch];
-  if (!a.dependent) {
+  if (!a.x_from_previous) {
     if constexpr (kFmt == 0)
       copy_x(item);
     else
@@ -516,8 +516,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   point();
 #pragma unroll
   for (int d = 0; d < kDepth; ++d) issue();
-  if (a.dependent) {
-    wait_for_previous_kernel();  // x is its output
+  if (a.x_from_previous) {
+    wait_for_previous_kernel();
     if constexpr (kFmt != 0)
       fetch_x(item, warp, first_x);
     else
@@ -821,7 +821,7 @@ cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
   const int unit_rows = (kGateUp ? 8 : 16) * (kWarps / a.k_warps);
   const long long most = static_cast<long long>(items) * ((a.rows + unit_rows - 1) / unit_rows);
   const int grid = static_cast<int>(most < slots ? most : slots);
-  return launch_kernel(kernel, dim3(grid), 32 * kWarps, smem, a.dependent != 0, stream, a);
+  return launch_kernel(kernel, dim3(grid), 32 * kWarps, smem, stream, a);
 }
 
 template <int kFmt, bool kGateUp>
@@ -863,7 +863,7 @@ cudaError_t launch_skinny(const SkinnyArgs& a, int group, bool gate_up, cudaStre
 
 cudaError_t launch_weighted_rows(const float* rows, const int32_t* indices, const float* weights, int tokens, int topk,
                                  int experts, int hidden, __nv_bfloat16* out, cudaStream_t stream) {
-  return launch_kernel(weighted_rows_kernel, dim3((hidden / 4 + 255) / 256, tokens), 256, 0, true, stream, rows, indices,
+  return launch_kernel(weighted_rows_kernel, dim3((hidden / 4 + 255) / 256, tokens), 256, 0, stream, rows, indices,
                        weights, topk, experts, hidden, out);
 }
 

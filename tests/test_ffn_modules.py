@@ -126,6 +126,44 @@ def test_swapped_experts_decode_in_4_bits():
 
 
 @gpu
+@pytest.mark.parametrize("T", [1, 20, 130])
+def test_calls_see_what_the_kernels_right_before_them_wrote(T):
+    """Inputs, weights, codes and expert ids written by kernels queued just before the call (which may start
+    under them): the results are those of a call made after everything has ended."""
+    H, F, E = 1024, 2048, 8
+    sets = []
+    for seed in (1, 2):
+        x, wg, wu, wd, _ = R.case(T, H, F, seed=seed, std=0.03)
+        t = min(T, 20)
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        idx = torch.randint(0, E, (t, 2), generator=gen, device="cuda").int()
+        sets.append([x, wg, wu, wd, *Q.codes((E, 2 * F, H), 64, seed), *Q.codes((E, H, F), 64, seed), idx,
+                     torch.rand(t, 2, generator=gen, device="cuda")])
+
+    def calls(v):
+        x, wg, wu, wd, q1, s1, q2, s2, idx, w = v
+        t = idx.shape[0]
+        return (cernels_b200.gated_ffn(x, wg, wu, wd), cernels_b200.linear_w4(x, q1[0], s1[0]),
+                cernels_b200.moe_experts_decode_w4(x[:t], q1, s1, q2, s2, idx, w, 2))
+
+    want = []
+    for v in sets:
+        torch.cuda.synchronize()
+        want.append([])
+        for i in range(3):
+            want[-1].append(calls(v)[i])
+            torch.cuda.synchronize()
+    live = [v.clone() for v in sets[0]]
+    for i in range(12):
+        for a, b in zip(live, sets[i % 2]):
+            a.copy_(b)
+        for a, b in zip(calls(live), want[i % 2]):
+            assert torch.equal(a, b)
+        x, wg, wu, wd = (v.detach().requires_grad_() for v in live[:4])  # and a training step after them
+        torch.autograd.grad(cernels_b200.gated_ffn(x, wg, wu, wd).sum(), (x, wg, wu, wd))
+
+
+@gpu
 def test_train_the_dense_block_then_decode_everything_in_a_graph():
     """A layer of a routed model in small: its shared block is trained for a few steps; then tokens are
     decoded from one graph: router, 4-bit experts, the shared block, a 4-bit output projection. The
