@@ -150,19 +150,25 @@ struct Item {
 // Buffers of the warps' sums: with two, a tile's additions overlap the next tile's products.
 __host__ __device__ constexpr int part_buffers(int warps) { return warps == 8 ? 2 : 1; }
 
+// Columns of the tile that `cols` columns are computed with.
+__host__ __device__ constexpr int tile_columns(bool bf16, int cols) {
+  return cols > 8 ? 16 : cols > 4 || bf16 ? 8 : 4;
+}
+
 struct SkinnySmem {
   size_t ring, part, units, x, items, ids, lead, count, first, sums, rank, list, order, total;
 };
 
-// blocks: of 128 values in padded_k (0 for bf16); pairs and experts: 0 without routing
-__host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int cols, int padded_k, int blocks, int pairs,
-                                                int experts) {
+// tile_cols: columns of the kernel's tile (its template argument), cols of them in use; blocks: of 128 values in
+// padded_k (0 for bf16); pairs and experts: 0 without routing
+__host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int tile_cols, int cols, int padded_k,
+                                                int blocks, int pairs, int experts) {
   SkinnySmem s;
   size_t off = 0;
   s.ring = off;
   off += static_cast<size_t>(warps) * kDepth * slot;
   s.part = off;
-  off += static_cast<size_t>(part_buffers(warps)) * warps * (cols > 8 ? 16 : cols > 4 ? 8 : 4) * 16 * 4;
+  off += static_cast<size_t>(part_buffers(warps)) * warps * tile_cols * 16 * 4;
   s.units = off;  // per column and block: 2^e / 16
   off += (static_cast<size_t>(blocks) * cols * 4 + 15) / 16 * 16;
   s.x = off;
@@ -287,7 +293,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   const int padded_k = steps * F::kStep;
   const int x_bytes = x_row_bytes(padded_k);
   const bool routed = a.indices != nullptr;
-  const SkinnySmem lay = carve_smem(kWarps, F::kSlot, a.cols, padded_k, kFmt == 0 ? 0 : padded_k / 128,
+  const SkinnySmem lay = carve_smem(kWarps, F::kSlot, kCols, a.cols, padded_k, kFmt == 0 ? 0 : padded_k / 128,
                                     routed ? a.pairs : 0, routed ? a.experts : 0);
   float* part = reinterpret_cast<float*>(smem + lay.part);
   const int blocks = padded_k / 128;
@@ -767,13 +773,13 @@ __global__ void __launch_bounds__(256) weighted_rows_kernel(const float* rows, c
   *reinterpret_cast<uint2*>(out + t * hidden + h) = v;
 }
 
-template <int kFmt>
+template <int kFmt, int kCols>
 size_t smem_bytes(const SkinnyArgs& a, int warps) {
   const int step = Format<kFmt>::kStep;
   const int padded = (a.k + step - 1) / step * step;
   const bool routed = a.indices != nullptr;
-  return carve_smem(warps, Format<kFmt>::kSlot, a.cols, padded, kFmt == 0 ? 0 : padded / 128, routed ? a.pairs : 0,
-                    routed ? a.experts : 0)
+  return carve_smem(warps, Format<kFmt>::kSlot, kCols, a.cols, padded, kFmt == 0 ? 0 : padded / 128,
+                    routed ? a.pairs : 0, routed ? a.experts : 0)
       .total;
 }
 
@@ -783,7 +789,7 @@ cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream);
 // Eight warps a CTA and two CTAs an SM; where x rows leave room for one, sixteen warps if they fit.
 template <int kFmt, bool kGateUp, int kCols>
 cudaError_t launch_tile(const SkinnyArgs& a, cudaStream_t stream) {
-  const size_t two = smem_bytes<kFmt>(a, 8), one = smem_bytes<kFmt>(a, 16);
+  const size_t two = smem_bytes<kFmt, kCols>(a, 8), one = smem_bytes<kFmt, kCols>(a, 16);
   return 2 * (two + 1024) > kSmemPerSm && one <= kMaxSmem ? launch_warps<kFmt, kGateUp, kCols, 16>(a, stream)
                                                           : launch_warps<kFmt, kGateUp, kCols, 8>(a, stream);
 }
@@ -794,7 +800,7 @@ cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
   const int step = Format<kFmt>::kStep;
   const int steps = (a.k + step - 1) / step;
   const bool routed = a.indices != nullptr;
-  const size_t smem = smem_bytes<kFmt>(a, kWarps);
+  const size_t smem = smem_bytes<kFmt, kCols>(a, kWarps);
   if (smem > kMaxSmem) return cudaErrorInvalidValue;
   static PerDeviceOnce attr;
   cudaError_t err =
@@ -826,9 +832,10 @@ cudaError_t launch_warps(SkinnyArgs a, cudaStream_t stream) {
 
 template <int kFmt, bool kGateUp>
 cudaError_t launch_columns(const SkinnyArgs& a, cudaStream_t stream) {
+  const int cols = tile_columns(kFmt == 0, a.cols);
   if constexpr (kFmt != 0)
-    if (a.cols <= 4) return launch_tile<kFmt, kGateUp, 4>(a, stream);
-  if (a.cols <= 8) return launch_tile<kFmt, kGateUp, 8>(a, stream);
+    if (cols == 4) return launch_tile<kFmt, kGateUp, 4>(a, stream);
+  if (cols == 8) return launch_tile<kFmt, kGateUp, 8>(a, stream);
   if constexpr (kFmt == 0 || !kGateUp) return launch_tile<kFmt, kGateUp, 16>(a, stream);
   return cudaErrorInvalidValue;  // 4-bit gate/up products are the experts', at most 8 columns
 }
@@ -851,7 +858,9 @@ int skinny_columns(int want, int k, int group, int pairs, int experts) {
   const int slot = group == 0 ? Format<0>::kSlot : group == 128 ? Format<128>::kSlot : group == 64 ? Format<64>::kSlot : Format<32>::kSlot;
   const int padded = (k + step - 1) / step * step;
   int cols = want < kSkinnyMaxColumns ? want : kSkinnyMaxColumns;
-  while (cols > 0 && carve_smem(8, slot, cols, padded, group == 0 ? 0 : padded / 128, pairs, experts).total > kMaxSmem)
+  const int blocks = group == 0 ? 0 : padded / 128;
+  while (cols > 0 &&
+         carve_smem(8, slot, tile_columns(group == 0, cols), cols, padded, blocks, pairs, experts).total > kMaxSmem)
     --cols;
   return cols;
 }

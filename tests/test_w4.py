@@ -103,7 +103,9 @@ def test_c_experts_refuse_shapes(shape, group, code):
 @gpu
 @pytest.mark.parametrize("group", [32, 64, 128])
 @pytest.mark.parametrize("T,N,groups", [(1, 1, 1), (1, 16, 4), (2, 17, 3), (3, 100, 9), (7, 250, 16), (8, 64, 33), (9, 33, 5),
-                                        (16, 130, 8), (17, 40, 7), (33, 31, 2), (1, 5000, 8), (5, 9000, 3)])
+                                        (16, 130, 8), (17, 40, 7), (33, 31, 2), (1, 5000, 8), (5, 9000, 3),
+                                        # more tiles than a CTA takes at once, for each kernel by columns
+                                        (1, 90000, 2), (4, 50001, 3), (7, 60000, 2), (13, 50000, 2), (20, 30000, 2)])
 def test_linear(T, N, groups, group):
     K = groups * group
     x = rows(T, K, T + N)
@@ -189,7 +191,8 @@ def test_linear_refusals():
 @pytest.mark.parametrize("T,H,E,F,k,group", [
     (1, 64, 4, 32, 2, 32), (1, 128, 1, 64, 1, 64), (2, 256, 8, 128, 3, 128), (5, 96, 3, 160, 3, 32), (8, 192, 16, 64, 4, 64),
     (9, 128, 2, 128, 1, 128), (16, 256, 64, 384, 6, 128), (29, 64, 7, 96, 2, 32), (64, 128, 300, 64, 8, 64),
-    (40, 64, 2, 32, 2, 32), (1, 2048, 64, 1408, 6, 128)])
+    (40, 64, 2, 32, 2, 32), (1, 2048, 64, 1408, 6, 128), (12, 256, 6, 8192, 2, 64), (3, 8192, 4, 128, 2, 32),
+    (40, 128, 3, 4096, 2, 128)])
 def test_experts(T, H, E, F, k, group):
     x = rows(T, H, T + H)
     w = experts(E, H, F, group, T + E)
