@@ -41,20 +41,30 @@ size_t act_bytes(const cernels_ffn_shape* s) {
   return align_up(static_cast<size_t>(s->tokens) * s->intermediate * 2, 256);
 }
 
-// A few tokens: the weights' bytes bound the work. The kernel that streams them reads them once per 16 tokens,
-// up to 48 from L2 where they fit half of it; the tile kernel takes a full tile's time for any number. (us,
-// streamed and tiled: H = F = 2880, 50 MB: 18.0 at 16 tokens, 24.5 and 30.3 at 48, 36.0 and 30.3 at 64; H = 4096,
-// F = 8192, 201 MB: 54.4 at 16, 64.8 and 62.8 at 24.)
-bool few(const cernels_ffn_shape* s) {
-  const long long weights = 6ll * s->hidden * s->intermediate;
-  return s->tokens <= kSkinnyMaxColumns || (s->tokens <= 48 && weights <= (64ll << 20));
+// Times that the weights are read for `tokens` rows of `k`; 0 when not even one row fits.
+int passes_of(int tokens, int k, int group) {
+  const int most = skinny_columns(kSkinnyMaxColumns, k, group, 0, 0);
+  return most == 0 ? 0 : (tokens + most - 1) / most;
 }
 
 int balanced_columns(int tokens, int k, int group) {
-  const int most = skinny_columns(kSkinnyMaxColumns, k, group, 0, 0);
-  if (most == 0) return 0;
-  const int passes = (tokens + most - 1) / most;
-  return (tokens + passes - 1) / passes;
+  const int passes = passes_of(tokens, k, group);
+  return passes == 0 ? 0 : (tokens + passes - 1) / passes;
+}
+
+// A few tokens: the weights' bytes bound the work, and the kernel that streams them (once per 16 tokens, or as
+// many as shared memory holds) beats the tile kernel, whose time is a full tile's for any number. By how much
+// more than once it may read them depends on whether L2 keeps them. us, streamed / tiled, at that many reads:
+//   50 MB (2880 x 2880)     3.0: 24.5 / 30.3   4.0: 36.0 / 30.3
+//   100 MB (8192 x 2048)    2.7: 35.4 / 48.0   3.3: 48.0 / 45.3     (4096 x 4096)  2.0: 39.2 / 38.3   3.0: 47.9 / 38.8
+//   302 MB (6144 x 8192)    1.0: 59.0 / 84.5   2.0: 80.2 / 72.0     402 MB (4096 x 16384)  1.7: 92.3 / 129.4
+bool few(const cernels_ffn_shape* s) {
+  if (s->tokens > 4 * kSkinnyMaxColumns) return false;
+  const int gate_up = passes_of(s->tokens, s->hidden, 0), down = passes_of(s->tokens, s->intermediate, 0);
+  if (gate_up == 0 || down == 0) return false;
+  const long long weights = 6ll * s->hidden * s->intermediate;
+  const int thirds = 2 * gate_up + down;  // of the weights' bytes that are read
+  return thirds <= (weights <= (64ll << 20) ? 9 : weights <= (105ll << 20) ? 8 : 5);
 }
 
 int check_group(int group, int a, int b) {
@@ -124,7 +134,7 @@ int cernels_gated_ffn(const cernels_ffn_shape* shape, const void* x, int64_t x_s
   if (!aligned(out) || !aligned(workspace)) return CERNELS_E_ALIGNMENT;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const FfnShape s = shape_of(shape);
-  if (few(shape) && skinny_columns(1, s.hidden, 0, 0, 0) && skinny_columns(1, s.inter, 0, 0, 0)) {
+  if (few(shape)) {
     SkinnyArgs a{};
     a.x = in(x);
     a.x_stride = static_cast<size_t>(x_stride);
