@@ -96,9 +96,11 @@ def _linear_family(cls_name: str):
                 if type(mod).__name__ == cls_name:
                     moe_experts_w4.release(mod)
             return plain(model, variant)
-        for mod in model.modules():
-            if type(mod).__name__ == cls_name:
-                moe_experts_w4.prepare(mod)
+        mods = [m for m in model.modules() if type(m).__name__ == cls_name]
+        for mod in mods:  # all of them or none
+            moe_experts_w4.group_of(mod.gate_up_proj.shape[2], mod.down_proj.shape[2])
+        for mod in mods:
+            moe_experts_w4.prepare(mod)
         return swap_experts(model, cls_name, _linear_kernels()[0], moe_experts_w4.decode_kernel)
 
     return apply
@@ -113,11 +115,13 @@ def swap_mlps(model: torch.nn.Module, cls_name: str, custom: bool) -> int:
     mods = [m for m in model.modules() if type(m).__name__ == cls_name]
     if not mods:
         raise RuntimeError(f"no {cls_name} modules found — wrong model for this swap")
+    if custom:  # all of them or none
+        for mod in mods:
+            gated_ffn.check_module(mod)
     for mod in mods:
         if "forward" in vars(mod):
             del mod.forward
         if custom:
-            gated_ffn.check_module(mod)
             mod.forward = lambda x, _m=mod: gated_ffn.kernel(x, _m)
     return len(mods)
 

@@ -63,6 +63,17 @@ def test_mlp_swap_sets_and_restores():
         swaps.SWAPS["qwen3_next_mlp"][0](m, "custom")
 
 
+def test_a_refused_swap_changes_nothing():
+    m = torch.nn.ModuleList([DeepseekV2MLP(), DeepseekV2MLP(bias=True)])
+    with pytest.raises(RuntimeError, match="bias"):
+        swaps.SWAPS["deepseek_v2_mlp"][0](m, "custom")
+    assert not any("forward" in vars(mod) for mod in m)
+    m = torch.nn.ModuleList([DeepseekV2Experts(), DeepseekV2Experts(hidden=48)])
+    with pytest.raises(RuntimeError, match="multiples"):
+        swaps.SWAPS["deepseek_v2"][0](m, "custom_w4")
+    assert not any(hasattr(mod, "_cernels_w4") or "forward" in vars(mod) for mod in m)
+
+
 def test_w4_copies_are_prepared_and_released():
     e = DeepseekV2Experts()
     with pytest.raises(RuntimeError, match="prepare"):
