@@ -12,6 +12,8 @@ caching allocator and never synchronises.
 from __future__ import annotations
 
 import ctypes
+import functools
+from typing import NamedTuple
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -27,7 +29,34 @@ def rows_ok(x: torch.Tensor) -> bool:
     return x.stride(1) == 1 and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0))
 
 
-def _validate(x, gate_proj, up_proj, down_proj) -> _lib.FfnShape:
+def int32_sizes(*sizes: int) -> None:
+    """Refuses sizes that the C ABI's 32-bit fields would wrap."""
+    _check(max(sizes) < 1 << 31, "sizes must be below 2^31")
+
+
+class _Plan(NamedTuple):
+    shape: _lib.FfnShape
+    ref: object  # ctypes.byref(shape)
+    workspace: int  # bytes
+    backward_workspace: int
+    saved: int
+
+
+@functools.lru_cache(maxsize=1024)
+def _plan(tokens: int, hidden: int, intermediate: int) -> _Plan:
+    """What the C ABI says about a call of these sizes (its queries are a few us of a 10 us call)."""
+    int32_sizes(tokens, hidden, intermediate)
+    shape = _lib.FfnShape(tokens, hidden, intermediate)
+    ref, lib, n = ctypes.byref(shape), _lib.load(), ctypes.c_size_t(0)
+    sizes = []
+    for backward in (0, 1):
+        _lib.check(lib.cernels_gated_ffn_workspace_bytes(ref, backward, ctypes.byref(n)), "workspace query")
+        sizes.append(n.value)
+    _lib.check(lib.cernels_gated_ffn_saved_bytes(ref, ctypes.byref(n)), "size query")
+    return _Plan(shape, ref, *sizes, n.value)
+
+
+def _validate(x, gate_proj, up_proj, down_proj) -> _Plan:
     _check(x.is_cuda, "x must be a CUDA tensor")
     _check(x.dim() == 2 and x.dtype is _BF16, "x must be [T, H] bf16")
     T, H = x.shape
@@ -41,7 +70,7 @@ def _validate(x, gate_proj, up_proj, down_proj) -> _lib.FfnShape:
     _check(down_proj.shape == (H, F), "down_proj must be [H, F]")
     _check(H > 0 and F > 0 and H % 8 == 0 and F % 8 == 0, "H and F must be multiples of 8")
     _check(rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least H) apart")
-    return _lib.FfnShape(T, H, F)
+    return _plan(T, H, F)
 
 
 def _stride(x: torch.Tensor) -> int:
@@ -67,34 +96,28 @@ def _call(device: torch.device, name: str, *args) -> None:
 
 
 def _forward(x, gate_proj, up_proj, down_proj) -> torch.Tensor:
-    shape = _validate(x, gate_proj, up_proj, down_proj)
-    out = x.new_empty((shape.tokens, shape.hidden))
-    if shape.tokens == 0:
+    plan = _validate(x, gate_proj, up_proj, down_proj)
+    out = x.new_empty(x.shape)
+    if x.shape[0] == 0:
         return out
-    n = ctypes.c_size_t(0)
-    _lib.check(_lib.load().cernels_gated_ffn_workspace_bytes(ctypes.byref(shape), 0, ctypes.byref(n)), "workspace query")
-    ws = x.new_empty((n.value + 1) // 2)
-    _call(x.device, "cernels_gated_ffn", ctypes.byref(shape), x.data_ptr(), _stride(x), gate_proj.data_ptr(),
-          up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), ws.data_ptr(), n.value)
+    ws = x.new_empty((plan.workspace + 1) // 2)
+    _call(x.device, "cernels_gated_ffn", plan.ref, x.data_ptr(), _stride(x), gate_proj.data_ptr(),
+          up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), ws.data_ptr(), plan.workspace)
     return out
 
 
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_proj, up_proj, down_proj):
-        shape = _validate(x, gate_proj, up_proj, down_proj)
-        T, F, dev = shape.tokens, shape.intermediate, x.device
-        out = x.new_empty((T, shape.hidden))
-        act = x.new_empty((T, F))
-        n = ctypes.c_size_t(0)
-        _lib.check(_lib.load().cernels_gated_ffn_saved_bytes(ctypes.byref(shape), ctypes.byref(n)), "size query")
-        saved = torch.empty(n.value // 4, dtype=torch.float32, device=dev)
-        if T:
-            _call(dev, "cernels_gated_ffn_forward", ctypes.byref(shape), x.data_ptr(), _stride(x),
-                  gate_proj.data_ptr(), up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), act.data_ptr(),
-                  saved.data_ptr())
+        plan = _validate(x, gate_proj, up_proj, down_proj)
+        out = x.new_empty(x.shape)
+        act = x.new_empty((plan.shape.tokens, plan.shape.intermediate))
+        saved = x.new_empty(plan.saved // 4, dtype=torch.float32)
+        if plan.shape.tokens:
+            _call(x.device, "cernels_gated_ffn_forward", plan.ref, x.data_ptr(), _stride(x), gate_proj.data_ptr(),
+                  up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), act.data_ptr(), saved.data_ptr())
         ctx.save_for_backward(x, gate_proj, up_proj, down_proj, act, saved)
-        ctx.shape = shape
+        ctx.plan = plan
         return out
 
     @staticmethod
@@ -106,20 +129,16 @@ class _GatedFfn(torch.autograd.Function):
 
 def _backward(ctx, dout):
     x, gate_proj, up_proj, down_proj, act, saved = ctx.saved_tensors
-    shape = ctx.shape
-    dev = x.device
+    plan = ctx.plan
     dout = dout.contiguous()
     if dout.data_ptr() % 16:
         dout = dout.clone()
     grads = [dout.new_empty(t.shape) if need else None
              for t, need in zip((x, gate_proj, up_proj, down_proj), ctx.needs_input_grad)]
-    n = ctypes.c_size_t(0)
-    _lib.check(_lib.load().cernels_gated_ffn_workspace_bytes(ctypes.byref(shape), 1, ctypes.byref(n)),
-               "workspace query")
-    ws = dout.new_empty((n.value + 1) // 2)
-    _call(dev, "cernels_gated_ffn_backward", ctypes.byref(shape), x.data_ptr(), _stride(x), gate_proj.data_ptr(),
+    ws = dout.new_empty((plan.backward_workspace + 1) // 2)
+    _call(x.device, "cernels_gated_ffn_backward", plan.ref, x.data_ptr(), _stride(x), gate_proj.data_ptr(),
           up_proj.data_ptr(), down_proj.data_ptr(), act.data_ptr(), saved.data_ptr(), dout.data_ptr(),
-          *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), n.value)
+          *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), plan.backward_workspace)
     return tuple(grads)
 
 

@@ -14,11 +14,12 @@ decode call (``*_moe_experts_decode``) on such weights, a quarter of the bytes t
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
 from . import _lib
-from .ffn import _call, rows_ok, _stride
+from .ffn import _call, int32_sizes, rows_ok, _stride
 from .ops import DECODE_MAX_PAIRS, _check
 
 _BF16 = torch.bfloat16
@@ -68,6 +69,7 @@ def _linear_w4(x, qweight, scales):
     _check(rows_ok(x), "x must have contiguous rows, a multiple of 8 elements (and at least K) apart")
     if scales.data_ptr() % 4:  # rows of a slice may start in the middle of the words that the kernel copies
         scales = scales.clone()
+    int32_sizes(T, N, K)
     out = x.new_empty((T, N))
     if T and N:
         _call(x.device, "cernels_linear_w4", T, N, K, group, x.data_ptr(), _stride(x), qweight.data_ptr(),
@@ -81,6 +83,15 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor) -> t
     read the weights once per 16."""
     _check_no_grad(x, scales)
     return _linear_w4(x, qweight, scales)
+
+
+@functools.lru_cache(maxsize=1024)
+def _moe_plan(tokens: int, hidden: int, experts: int, inter: int, topk: int, group: int):
+    """The C ABI's shape (kept alive by the reference to it that is returned) and workspace bytes."""
+    int32_sizes(tokens, hidden, experts, inter, topk)
+    ref, n = ctypes.byref(_lib.MoeShape(tokens, hidden, experts, inter, topk, _lib.LAYOUT_LINEAR)), ctypes.c_size_t(0)
+    _lib.check(_lib.load().cernels_moe_w4_workspace_bytes(ref, group, ctypes.byref(n)), "workspace query")
+    return ref, n.value
 
 
 def _moe_experts_decode_w4(x, gate_up_q, gate_up_scales, down_q, down_scales, indices, weights, topk):
@@ -99,14 +110,11 @@ def _moe_experts_decode_w4(x, gate_up_q, gate_up_scales, down_q, down_scales, in
     out = x.new_empty((T, H))
     if T == 0:
         return out
-    shape = _lib.MoeShape(T, H, E, F, topk, _lib.LAYOUT_LINEAR)
-    n = ctypes.c_size_t(0)
-    _lib.check(_lib.load().cernels_moe_w4_workspace_bytes(ctypes.byref(shape), group, ctypes.byref(n)),
-               "workspace query")
-    ws = x.new_empty((n.value + 1) // 2)
-    _call(x.device, "cernels_moe_experts_decode_w4", ctypes.byref(shape), group, x.data_ptr(), gate_up_q.data_ptr(),
+    ref, n = _moe_plan(T, H, E, F, topk, group)
+    ws = x.new_empty((n + 1) // 2)
+    _call(x.device, "cernels_moe_experts_decode_w4", ref, group, x.data_ptr(), gate_up_q.data_ptr(),
           gate_up_scales.data_ptr(), down_q.data_ptr(), down_scales.data_ptr(), indices.data_ptr(), weights.data_ptr(),
-          out.data_ptr(), ws.data_ptr(), n.value)
+          out.data_ptr(), ws.data_ptr(), n)
     return out
 
 

@@ -50,6 +50,12 @@ def test_c_entry_refuses_shapes(bad, code):
     assert lib.cernels_gated_ffn_saved_bytes(ctypes.byref(s), ctypes.byref(n)) == code
 
 
+@pytest.mark.parametrize("sizes", [(2**32 + 1, 8, 8), (1, 2**31, 8), (1, 8, 2**32 + 8)])
+def test_sizes_do_not_wrap(sizes):
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        ffn._plan(*sizes)
+
+
 def test_c_entry_refuses_pointers():
     import ctypes
 

@@ -6,7 +6,7 @@ import pytest
 import torch
 
 import cernels_b200
-from cernels_b200 import _lib
+from cernels_b200 import _lib, w4
 from tests import w4_reference as R
 from tests.ffn_reference import assert_within
 
@@ -97,6 +97,12 @@ def test_c_linear_refuses_pointers():
 def test_c_experts_refuse_shapes(shape, group, code):
     s, n = _lib.MoeShape(*shape), ctypes.c_size_t(0)
     assert _lib.load().cernels_moe_w4_workspace_bytes(ctypes.byref(s), group, ctypes.byref(n)) == code
+
+
+@pytest.mark.parametrize("sizes", [(2**32 + 1, 64, 4, 32, 2), (1, 64, 4, 2**32 + 32, 2), (1, 64, 2**32 + 4, 32, 2)])
+def test_sizes_do_not_wrap(sizes):
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        w4._moe_plan(*sizes, 32)
 
 
 # ---------------------------------------------------------------- GPU: linear
