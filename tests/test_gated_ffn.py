@@ -14,7 +14,9 @@ gpu = pytest.mark.gpu
 # divides, widths under one K block, several tiles each way
 SHAPES = [(1, 64, 64), (2, 8, 8), (5, 72, 40), (16, 256, 136), (17, 2048, 512), (31, 200, 264), (33, 64, 72), (48, 72, 520), (49, 72, 520), (20, 16384, 8), (20, 8, 16384), (3, 65536, 8),
           # more tiles than a CTA takes at once, at every number of columns that has a kernel of its own
-          (1, 64, 40000), (4, 40000, 64), (3, 4096, 8192), (9, 72, 40000), (13, 2880, 2880), (16, 40000, 72), (33, 64, 20000), (127, 328, 128),
+          (1, 64, 40000), (4, 40000, 64), (3, 4096, 8192), (9, 72, 40000), (13, 2880, 2880), (16, 40000, 72), (33, 64, 20000),
+          # rows of x that shared memory does not hold
+          (2, 131072, 8), (1, 8, 131072), (127, 328, 128),
           (128, 64, 192), (129, 520, 384), (255, 136, 264), (257, 1024, 520), (512, 768, 256), (700, 2880, 328),
           (1300, 136, 1408)]
 
