@@ -26,6 +26,7 @@
 #include <cmath>
 
 #include "ffn_internal.h"
+#include "pair_drain.h"
 #include "pair_gemm.cuh"
 
 namespace cernels {
@@ -130,6 +131,18 @@ __device__ __forceinline__ void stage(uint8_t* window, int lane, int col, const 
   }
 }
 
+// Waits until every load has landed that the CTAs of the pair started (pair_drain.h), kBytes a block and CTA. CTA 0.
+template <int kStages, int kBytes>
+__device__ void drain_loads(uint64_t* full_bar, long long mine, long long other) {
+  for (long long i = drain_first(mine, other, kStages); i < max(mine, other); ++i) {
+    uint64_t* bar = &full_bar[i % kStages];
+    const Drain action = drain_action(i, mine, other);
+    if (action == Drain::kAnnounce) mbar_arrive_expect_tx(bar, kBytes);
+    if (action == Drain::kCancel) mbar_complete_tx(bar, kBytes);
+    mbar_drain(bar, static_cast<uint32_t>((i / kStages) & 1), kWaitLimitNs);
+  }
+}
+
 template <int kEpi, int BN>
 __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     pair_gemm_kernel(const __grid_constant__ Maps maps, const __grid_constant__ PairArgs args) {
@@ -148,6 +161,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
   uint64_t* drain_bar = tempty_bar + 2;       // [1]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  volatile long long* issued_count = reinterpret_cast<volatile long long*>(tmem_slot + 2);  // K blocks whose loads started
+  volatile int* peer_abort = reinterpret_cast<volatile int*>(tmem_slot + 4);  // the other CTA's abort_flag, when it is over
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
@@ -166,6 +181,8 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
+    *issued_count = 0;
+    *peer_abort = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -225,12 +242,7 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           }
         }
       }
-      if (!ok && rank == 0) {
-        // Giving up: CTA 0's barriers count both CTAs' loads; let those in flight land before the
-        // pair_sync() below lets either CTA exit.
-        for (long long i = issued > kStages ? issued - kStages : 0; i < issued; ++i)
-          mbar_drain(&full_bar[i % kStages], static_cast<uint32_t>((i / kStages) & 1), args.wait_ns);
-      }
+      *issued_count = issued;
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -274,10 +286,6 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
           }
         }
         if (ok) umma_commit_pair(&tfull_bar[acc]);
-      }
-      if (*abort_flag) {  // let the MMAs in flight finish before the TMEM is freed
-        umma_commit_pair(drain_bar);
-        mbar_drain(drain_bar, 0, args.wait_ns);
       }
     }
     __syncwarp();
@@ -410,7 +418,25 @@ __global__ void __launch_bounds__(kThreads, 1) __cluster_dims__(2, 1, 1)
 
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && *abort_flag) store_peer(peer_abort, rank ^ 1u, 1);
+  __syncwarp();
   pair_sync();  // neither CTA leaves while the other may still reach its shared memory or TMEM
+  // A wait gave up, whichever role's and in whichever CTA (both see the same here): loads and MMAs that it did
+  // not wait for may be in flight in both CTAs. They end within this kernel, however short the limit of its waits.
+  if (*abort_flag != 0 || *peer_abort != 0) {
+    if (warp == 1) {
+      if (elect_one()) {
+        if (rank == 0) {
+          umma_commit_pair(drain_bar);  // of the thread that issued the MMAs: elect_one() has one answer per warp
+          drain_loads<kStages, C::kStageBytes>(full_bar, *issued_count, load_peer(issued_count, 1));
+        }
+        mbar_drain(drain_bar, 0, kWaitLimitNs);
+      }
+      __syncwarp();
+    }
+    __syncthreads();
+    pair_sync();
+  }
   if (warp == 1) {
     tc_fence_after();
     tmem_dealloc_pair(tmem_base, 2 * BN);

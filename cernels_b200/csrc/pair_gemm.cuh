@@ -23,6 +23,33 @@ __device__ __forceinline__ uint32_t leader_smem(const void* p) {
   return r;
 }
 
+// A word of the other CTA's shared memory, at the place that `p` has in this one's.
+__device__ __forceinline__ void store_peer(const volatile int* p, uint32_t peer, int v) {
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %0, %1;\n\t"
+      "st.shared::cluster.u32 [a], %2;\n\t}" ::"r"(smem_u32(const_cast<const int*>(p))),
+      "r"(peer), "r"(v)
+      : "memory");
+}
+__device__ __forceinline__ long long load_peer(const volatile long long* p, uint32_t peer) {
+  long long v;
+  asm volatile(
+      "{\n\t.reg .b32 a;\n\t"
+      "mapa.shared::cluster.u32 a, %1, %2;\n\t"
+      "ld.shared::cluster.u64 %0, [a];\n\t}"
+      : "=l"(v)
+      : "r"(smem_u32(const_cast<const long long*>(p))), "r"(peer)
+      : "memory");
+  return v;
+}
+
+// Takes `bytes` off what the barrier's current phase still expects.
+__device__ __forceinline__ void mbar_complete_tx(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
+               : "memory");
+}
+
 __device__ __forceinline__ void mbar_arrive_leader(uint32_t leader_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader_bar) : "memory");
 }
