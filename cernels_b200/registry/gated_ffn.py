@@ -12,17 +12,41 @@ import torch
 from ..ffn import gated_ffn, rows_ok
 
 
+_PROJECTIONS = ("gate_proj", "up_proj", "down_proj")
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _altered(mod) -> bool:
+    """Whether calling `mod` does more than its class's forward: hooks, or a forward of its own."""
+    d = vars(mod)
+    return "forward" in d or any(d.get(h) for h in _HOOKS)
+
+
+def _is_silu(act) -> bool:
+    if act is torch.nn.functional.silu:
+        return True
+    kind = type(act)
+    known = kind is torch.nn.SiLU or (kind.__name__ == "SiLUActivation" and kind.__module__ == "transformers.activations")
+    return known and not _altered(act)
+
+
 def check_module(mlp) -> None:
-    """Raises when `mlp` computes something else than down(silu(gate(x)) * up(x)) without biases."""
+    """Raises when `mlp` computes something else than down(silu(gate(x)) * up(x)) without biases, as far as its
+    parts show: projections that are not torch.nn.Linear itself (adapters, parametrisations, quantised layers) or carry
+    hooks, which the operator would pass by, and an activation that is not SiLU."""
     if mlp is None:
         raise RuntimeError("mlp module not available (meta device)")
-    for name in ("gate_proj", "up_proj", "down_proj"):
-        if getattr(mlp, name).bias is not None:
+    for name in _PROJECTIONS:
+        proj = getattr(mlp, name)
+        if type(proj) is not torch.nn.Linear:
+            raise RuntimeError(f"gated_ffn takes plain torch.nn.Linear projections: {name} is {type(proj).__name__}")
+        if proj.bias is not None:
             raise RuntimeError(f"gated_ffn has no bias: {name} has one")
+        if _altered(proj):
+            raise RuntimeError(f"gated_ffn does not call its projections: {name} has hooks or a forward of its own")
     act = getattr(mlp, "act_fn", None)
-    if act is not None and not isinstance(act, torch.nn.SiLU) and getattr(act, "__name__", "") != "silu":
-        if type(act).__name__ not in ("SiLU", "SiLUActivation"):
-            raise RuntimeError(f"gated_ffn applies silu, the module {type(act).__name__}")
+    if not _is_silu(act):
+        raise RuntimeError(f"gated_ffn applies silu, the module {getattr(act, '__name__', type(act).__name__)}")
 
 
 def kernel(x, mlp):

@@ -1,0 +1,114 @@
+"""Which modules the gated block's loader and swap take: those that compute what the operator computes."""
+
+import pytest
+import torch
+
+from cernels_b200 import swaps
+from cernels_b200.registry import gated_ffn
+from tests.test_ffn_modules import DeepseekV2MLP
+
+
+class Adapter(torch.nn.Module):  # a low-rank adapter that shows its base layer's weight and bias
+    def __init__(self, base):
+        super().__init__()
+        self.base = base
+        self.a = torch.nn.Parameter(torch.randn(4, base.in_features))
+        self.b = torch.nn.Parameter(torch.randn(base.out_features, 4))
+
+    weight = property(lambda self: self.base.weight)
+    bias = property(lambda self: self.base.bias)
+
+    def forward(self, x):
+        return self.base(x) + x @ self.a.T @ self.b.T
+
+
+class Wider(torch.nn.Linear):
+    def forward(self, x):
+        return 2.0 * super().forward(x)
+
+
+def wrap(mlp, name):
+    setattr(mlp, name, Adapter(getattr(mlp, name)))
+
+
+def subclass(mlp, name):
+    setattr(mlp, name, Wider(64, 96, bias=False))
+
+
+def parametrised(mlp, name):
+    torch.nn.utils.parametrize.register_parametrization(getattr(mlp, name), "weight", torch.nn.Identity())
+
+
+def weight_norm(mlp, name):  # recomputes the weight in a hook before each call
+    proj = getattr(mlp, name)
+    proj.weight.data = proj.weight.data.float()
+    torch.nn.utils.weight_norm(proj)
+
+
+def forward_hook(mlp, name):
+    getattr(mlp, name).register_forward_hook(lambda mod, args, out: 2 * out)
+
+
+def pre_hook(mlp, name):
+    getattr(mlp, name).register_forward_pre_hook(lambda mod, args: (args[0] + 1,))
+
+
+def backward_hook(mlp, name):
+    getattr(mlp, name).register_full_backward_hook(lambda mod, gi, go: None)
+
+
+def own_forward(mlp, name):
+    proj = getattr(mlp, name)
+    proj.forward = lambda x: 3.0 * torch.nn.functional.linear(x, proj.weight)
+
+
+@pytest.mark.parametrize("name", ["gate_proj", "up_proj", "down_proj"])
+@pytest.mark.parametrize("change", [wrap, subclass, parametrised, weight_norm, forward_hook, pre_hook, backward_hook,
+                                    own_forward])
+def test_changed_projections_are_refused(change, name):
+    m = torch.nn.ModuleList([DeepseekV2MLP(), DeepseekV2MLP()])
+    change(m[1], name)
+    with pytest.raises(RuntimeError, match=name):
+        gated_ffn.check_module(m[1])
+    with pytest.raises(RuntimeError, match=name):
+        swaps.SWAPS["deepseek_v2_mlp"][0](m, "custom")
+    assert not any("forward" in vars(mod) for mod in m)
+
+
+@pytest.mark.parametrize("change", [wrap, forward_hook])
+def test_projections_changed_after_the_swap_are_refused_when_called(change):
+    m = torch.nn.ModuleList([DeepseekV2MLP()])
+    swaps.SWAPS["deepseek_v2_mlp"][0](m, "custom")
+    change(m[0], "up_proj")
+    with pytest.raises(RuntimeError, match="up_proj"):
+        m[0](torch.zeros(1, 64, dtype=torch.bfloat16))
+
+
+def test_activations():
+    def silu(x):  # another function of that name
+        return x
+
+    class Scaled(torch.nn.SiLU):
+        def forward(self, x):
+            return 2.0 * super().forward(x)
+
+    hooked = torch.nn.SiLU()
+    hooked.register_forward_hook(lambda mod, args, out: -out)
+    for act in (silu, Scaled(), hooked, torch.nn.GELU()):
+        with pytest.raises(RuntimeError, match="silu"):
+            gated_ffn.check_module(DeepseekV2MLP(act=act))
+    without = DeepseekV2MLP()
+    del without.act_fn
+    with pytest.raises(RuntimeError, match="silu"):  # whatever it applies, it is not known to be silu
+        gated_ffn.check_module(without)
+    gated_ffn.check_module(DeepseekV2MLP(act=torch.nn.SiLU(inplace=True)))
+
+
+def test_the_transformers_modules_are_taken():
+    transformers = pytest.importorskip("transformers")
+    from transformers.models.deepseek_v2.modeling_deepseek_v2 import DeepseekV2MLP as Deepseek
+    from transformers.models.qwen3_next.modeling_qwen3_next import Qwen3NextMLP as Qwen
+
+    small = dict(hidden_size=64, intermediate_size=96, hidden_act="silu")
+    for mlp in (Deepseek(transformers.DeepseekV2Config(**small)), Qwen(transformers.Qwen3NextConfig(**small), 96)):
+        gated_ffn.check_module(mlp)
