@@ -16,6 +16,7 @@ import functools
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -32,6 +33,13 @@ def rows_ok(x: torch.Tensor) -> bool:
 def int32_sizes(*sizes: int) -> None:
     """Refuses sizes that the C ABI's 32-bit fields would wrap."""
     _check(max(sizes) < 1 << 31, "sizes must be below 2^31")
+
+
+def refuse_tangents(name: str, *tensors: torch.Tensor) -> None:
+    """Raises for forward-mode inputs: the operators have no such derivative, and a tangent must not get lost."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            _check(forward_ad.unpack_dual(t).tangent is None, f"{name} has no forward-mode derivative")
 
 
 class _Plan(NamedTuple):
@@ -152,6 +160,7 @@ def gated_ffn(x: torch.Tensor, gate_proj: torch.Tensor, up_proj: torch.Tensor, d
     [F, H], down_proj [H, F], contiguous bf16; H and F multiples of 8. Sums run in 32 bits; the
     product of the halves is rounded to bf16 once, as the second matrix product's operand.
     """
+    refuse_tangents("gated_ffn", x, gate_proj, up_proj, down_proj)
     if torch.is_grad_enabled() and (x.requires_grad or gate_proj.requires_grad or up_proj.requires_grad
                                     or down_proj.requires_grad):
         return _GatedFfn.apply(x, gate_proj, up_proj, down_proj)

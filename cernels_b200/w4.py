@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _lib
-from .ffn import _call, int32_sizes, rows_ok, _stride
+from .ffn import _call, int32_sizes, refuse_tangents, rows_ok, _stride
 from .ops import DECODE_MAX_PAIRS, _check
 
 _BF16 = torch.bfloat16
@@ -40,6 +40,7 @@ def quantize_w4(weight: torch.Tensor, group: int = 128) -> tuple[torch.Tensor, t
 
 
 def _check_no_grad(*tensors: torch.Tensor) -> None:
+    refuse_tangents("a 4-bit product", *tensors)
     if torch.is_grad_enabled():
         for t in tensors:
             _check(not t.requires_grad, "4-bit products have no gradient: call them under torch.no_grad()")
