@@ -103,6 +103,30 @@ def _call(device: torch.device, name: str, *args) -> None:
         _lib.check(rc, name)
 
 
+_PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
+_compiling = torch.compiler.is_compiling
+_modes = torch._C._len_torch_dispatch_stack
+_transform = torch._C._functorch.peek_interpreter_stack
+
+
+def traced(*tensors: torch.Tensor) -> bool:
+    """Whether a call has to go through torch's dispatcher: tensors that stand for others (fake ones of torch.compile and
+    torch.export, wrappers), or a mode or transform that wants to see it. Else it launches at once: the way there and
+    back is a few us of a 10 us call."""
+    if _compiling() or _modes() or _transform() is not None:
+        return True
+    for t in tensors:
+        if type(t) not in _PLAIN:
+            return True
+    return False
+
+
+def below_autograd(op, *args):
+    """Calls `op` at the implementations below autograd's: a device's, Meta, or a tracer."""
+    with torch._C._AutoDispatchBelowAutograd():
+        return op(*args)
+
+
 def _forward(x, gate_proj, up_proj, down_proj) -> torch.Tensor:
     plan = _validate(x, gate_proj, up_proj, down_proj)
     out = x.new_empty(x.shape)
@@ -114,18 +138,41 @@ def _forward(x, gate_proj, up_proj, down_proj) -> torch.Tensor:
     return out
 
 
+def _train(x, gate_proj, up_proj, down_proj) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The result and what the backward pass reads: silu(g) * u in bf16, g and u in 32 bits (the kernels' order)."""
+    plan = _validate(x, gate_proj, up_proj, down_proj)
+    out = x.new_empty(x.shape)
+    act = x.new_empty((plan.shape.tokens, plan.shape.intermediate))
+    saved = x.new_empty(plan.saved // 4, dtype=torch.float32)
+    if plan.shape.tokens:
+        _call(x.device, "cernels_gated_ffn_forward", plan.ref, x.data_ptr(), _stride(x), gate_proj.data_ptr(),
+              up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), act.data_ptr(), saved.data_ptr())
+    return out, act, saved
+
+
+def _grads(dout, x, gate_proj, up_proj, down_proj, act, saved, needs) -> tuple[torch.Tensor | None, ...]:
+    """The gradients of the arguments that `needs` marks."""
+    plan = _plan(x.shape[0], x.shape[1], gate_proj.shape[0])
+    dout = dout.contiguous()
+    if dout.data_ptr() % 16:
+        dout = dout.clone()
+    grads = [dout.new_empty(t.shape) if need else None for t, need in zip((x, gate_proj, up_proj, down_proj), needs)]
+    ws = dout.new_empty((plan.backward_workspace + 1) // 2)
+    _call(x.device, "cernels_gated_ffn_backward", plan.ref, x.data_ptr(), _stride(x), gate_proj.data_ptr(),
+          up_proj.data_ptr(), down_proj.data_ptr(), act.data_ptr(), saved.data_ptr(), dout.data_ptr(),
+          *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), plan.backward_workspace)
+    return tuple(grads)
+
+
+def _grads_op(*args) -> list[torch.Tensor]:
+    return [g for g in _grads(*args) if g is not None]
+
+
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_proj, up_proj, down_proj):
-        plan = _validate(x, gate_proj, up_proj, down_proj)
-        out = x.new_empty(x.shape)
-        act = x.new_empty((plan.shape.tokens, plan.shape.intermediate))
-        saved = x.new_empty(plan.saved // 4, dtype=torch.float32)
-        if plan.shape.tokens:
-            _call(x.device, "cernels_gated_ffn_forward", plan.ref, x.data_ptr(), _stride(x), gate_proj.data_ptr(),
-                  up_proj.data_ptr(), down_proj.data_ptr(), out.data_ptr(), act.data_ptr(), saved.data_ptr())
+        out, act, saved = _train(x, gate_proj, up_proj, down_proj)
         ctx.save_for_backward(x, gate_proj, up_proj, down_proj, act, saved)
-        ctx.plan = plan
         return out
 
     @staticmethod
@@ -135,19 +182,20 @@ class _GatedFfn(torch.autograd.Function):
         return (_backward_recorded if torch.is_grad_enabled() else _backward)(ctx, dout)
 
 
+class _TracedGatedFfn(_GatedFfn):
+    @staticmethod
+    def forward(ctx, *t):
+        out, act, saved = below_autograd(_ops.gated_ffn_train, *t)
+        ctx.save_for_backward(*t, act, saved)
+        return out
+
+
 def _backward(ctx, dout):
-    x, gate_proj, up_proj, down_proj, act, saved = ctx.saved_tensors
-    plan = ctx.plan
-    dout = dout.contiguous()
-    if dout.data_ptr() % 16:
-        dout = dout.clone()
-    grads = [dout.new_empty(t.shape) if need else None
-             for t, need in zip((x, gate_proj, up_proj, down_proj), ctx.needs_input_grad)]
-    ws = dout.new_empty((plan.backward_workspace + 1) // 2)
-    _call(x.device, "cernels_gated_ffn_backward", plan.ref, x.data_ptr(), _stride(x), gate_proj.data_ptr(),
-          up_proj.data_ptr(), down_proj.data_ptr(), act.data_ptr(), saved.data_ptr(), dout.data_ptr(),
-          *(None if g is None else g.data_ptr() for g in grads), ws.data_ptr(), plan.backward_workspace)
-    return tuple(grads)
+    needs, saved = ctx.needs_input_grad, ctx.saved_tensors
+    if not traced(dout):
+        return _grads(dout, *saved, needs)
+    grads = iter(below_autograd(_ops.gated_ffn_backward, dout, *saved, needs))
+    return tuple(next(grads) if need else None for need in needs)
 
 
 _backward_recorded = once_differentiable(_backward)
@@ -160,15 +208,37 @@ def gated_ffn(x: torch.Tensor, gate_proj: torch.Tensor, up_proj: torch.Tensor, d
     [F, H], down_proj [H, F], contiguous bf16; H and F multiples of 8. Sums run in 32 bits; the
     product of the halves is rounded to bf16 once, as the second matrix product's operand.
     """
-    refuse_tangents("gated_ffn", x, gate_proj, up_proj, down_proj)
-    if torch.is_grad_enabled() and (x.requires_grad or gate_proj.requires_grad or up_proj.requires_grad
-                                    or down_proj.requires_grad):
+    if traced(x, gate_proj, up_proj, down_proj):
+        return _ops.gated_ffn(x, gate_proj, up_proj, down_proj)
+    if _records(x, gate_proj, up_proj, down_proj):
         return _GatedFfn.apply(x, gate_proj, up_proj, down_proj)
     return _forward(x, gate_proj, up_proj, down_proj)
 
 
+def _records(x, gate_proj, up_proj, down_proj) -> bool:
+    refuse_tangents("gated_ffn", x, gate_proj, up_proj, down_proj)
+    return torch.is_grad_enabled() and (x.requires_grad or gate_proj.requires_grad or up_proj.requires_grad
+                                        or down_proj.requires_grad)
+
+
+def _dispatched(*t):
+    if _records(*t):
+        return (_TracedGatedFfn if traced(*t) else _GatedFfn).apply(*t)
+    return below_autograd(_ops.gated_ffn, *t) if traced(*t) else _forward(*t)
+
+
 def _meta(x, gate_proj, up_proj, down_proj):
     return x.new_empty((x.shape[0], down_proj.shape[0]))
+
+
+def _meta_train(x, gate_proj, up_proj, down_proj):
+    T, F = x.shape[0], gate_proj.shape[0]
+    return (_meta(x, gate_proj, up_proj, down_proj), x.new_empty((T, F)),
+            x.new_empty((T + 31) // 32 * 32 * 2 * F, dtype=torch.float32))
+
+
+def _meta_grads(dout, x, gate_proj, up_proj, down_proj, act, saved, needs):
+    return [t.new_empty(t.shape) for t, need in zip((x, gate_proj, up_proj, down_proj), needs) if need]
 
 
 def status(device: torch.device | int | None = None) -> int:
@@ -184,7 +254,16 @@ def status(device: torch.device | int | None = None) -> int:
 
 
 _DEF = torch.library.Library("cernels_b200", "FRAGMENT")
-_DEF.define("gated_ffn(Tensor x, Tensor gate_proj, Tensor up_proj, Tensor down_proj) -> Tensor")
+_ARGS = "Tensor x, Tensor gate_proj, Tensor up_proj, Tensor down_proj"
+_DEF.define(f"gated_ffn({_ARGS}) -> Tensor")
+_DEF.define(f"gated_ffn_train({_ARGS}) -> (Tensor, Tensor, Tensor)")
+_DEF.define(f"gated_ffn_backward(Tensor dout, {_ARGS}, Tensor act, Tensor saved, bool[] needs) -> Tensor[]")
 _DEF.impl("gated_ffn", _forward, "CUDA")
-_DEF.impl("gated_ffn", gated_ffn, "AutogradCUDA")
+_DEF.impl("gated_ffn", _dispatched, "AutogradCUDA")
 _DEF.impl("gated_ffn", _meta, "Meta")
+# the halves of a training step, as a traced one records them
+_DEF.impl("gated_ffn_train", _train, "CUDA")
+_DEF.impl("gated_ffn_train", _meta_train, "Meta")
+_DEF.impl("gated_ffn_backward", _grads_op, "CUDA")
+_DEF.impl("gated_ffn_backward", _meta_grads, "Meta")
+_ops = torch.ops.cernels_b200

@@ -19,7 +19,7 @@ import functools
 import torch
 
 from . import _lib
-from .ffn import _call, int32_sizes, refuse_tangents, rows_ok, _stride
+from .ffn import _call, below_autograd, int32_sizes, refuse_tangents, rows_ok, _stride, traced
 from .ops import DECODE_MAX_PAIRS, _check
 
 _BF16 = torch.bfloat16
@@ -82,8 +82,16 @@ def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor) -> t
     """``x @ W.T`` for 4-bit W: x [T, K] bf16 (rows may lie apart), qweight [N, K / 2] uint8, scales
     [N, K / G] bf16. Made for up to 16 rows, where the weights' bytes bound it; more rows work, and
     read the weights once per 16."""
+    if traced(x, qweight, scales):
+        return _ops.linear_w4(x, qweight, scales)
     _check_no_grad(x, scales)
     return _linear_w4(x, qweight, scales)
+
+
+def _linear_dispatched(x, qweight, scales):
+    _check_no_grad(x, scales)
+    t = x, qweight, scales
+    return below_autograd(_ops.linear_w4, *t) if traced(*t) else _linear_w4(*t)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -127,8 +135,17 @@ def moe_experts_decode_w4(x: torch.Tensor, gate_up_q: torch.Tensor, gate_up_scal
     x [T, H] bf16; gate_up_q [E, 2F, H / 2], down_q [E, H, F / 2] uint8 with their scales; indices
     [T, topk] int32 (ids outside [0, E) are skipped), weights [T, topk] fp32. At most 1024 pairs.
     """
+    t = x, gate_up_q, gate_up_scales, down_q, down_scales, indices, weights
+    if traced(*t):
+        return _ops.moe_experts_decode_w4(*t, topk)
     _check_no_grad(x, gate_up_scales, down_scales, weights)
-    return _moe_experts_decode_w4(x, gate_up_q, gate_up_scales, down_q, down_scales, indices, weights, topk)
+    return _moe_experts_decode_w4(*t, topk)
+
+
+def _moe_dispatched(x, gate_up_q, gate_up_scales, down_q, down_scales, indices, weights, topk):
+    _check_no_grad(x, gate_up_scales, down_scales, weights)
+    t = x, gate_up_q, gate_up_scales, down_q, down_scales, indices, weights
+    return below_autograd(_ops.moe_experts_decode_w4, *t, topk) if traced(*t) else _moe_experts_decode_w4(*t, topk)
 
 
 _DEF = torch.library.Library("cernels_b200", "FRAGMENT")
@@ -136,8 +153,9 @@ _DEF.define("linear_w4(Tensor x, Tensor qweight, Tensor scales) -> Tensor")
 _DEF.define("moe_experts_decode_w4(Tensor x, Tensor gate_up_q, Tensor gate_up_scales, Tensor down_q, "
             "Tensor down_scales, Tensor indices, Tensor weights, int topk) -> Tensor")
 _DEF.impl("linear_w4", _linear_w4, "CUDA")
-_DEF.impl("linear_w4", linear_w4, "AutogradCUDA")
+_DEF.impl("linear_w4", _linear_dispatched, "AutogradCUDA")
 _DEF.impl("linear_w4", lambda x, qweight, scales: x.new_empty((x.shape[0], qweight.shape[0])), "Meta")
 _DEF.impl("moe_experts_decode_w4", _moe_experts_decode_w4, "CUDA")
-_DEF.impl("moe_experts_decode_w4", moe_experts_decode_w4, "AutogradCUDA")
+_DEF.impl("moe_experts_decode_w4", _moe_dispatched, "AutogradCUDA")
 _DEF.impl("moe_experts_decode_w4", lambda x, *rest: torch.empty_like(x), "Meta")
+_ops = torch.ops.cernels_b200
