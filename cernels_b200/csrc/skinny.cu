@@ -24,15 +24,23 @@
 // 128, x = 2^e v with |v| < 2^14, e from the block's largest |x|, as v = 256 hi + lo in two signed bytes and
 // two mma's (up to 4 columns: two columns of one mma). This keeps 14 bits below the block's largest value, where
 // bf16 x holds 8 bits of each value: every x within 2^-6 of the largest is exact, the others are rounded by at
-// most 2^-14 of it, far below the rounding of the output. The sums of 16 (q - 8) hi and 16 (q - 8) lo over a
+// most 2^-14 of it. That is far below the rounding of an output that the larger values enter, but the values between
+// a few large ones would be lost to an output whose weights are 0 where those stand. So a block of x in which more than half of
+// the nonzero values are under 128 units (2^-7 to 2^-6 of the largest) is mixed: it is not taken as integers but
+// multiplied in bf16, exactly, as are blocks with an infinity or a NaN (add_mixed: codes from L2 once more; where all
+// blocks are mixed a call takes 2 to 3 times as long, 18 -> 44 us for 16384 x 8192 at one row). In the
+// other blocks no x is off by more than 2^-8 of the median. Normal x has no mixed block, the halved products of normal
+// gates and ups one in a thousand.
+//
+// The sums of 16 (q - 8) hi and 16 (q - 8) lo over a
 // group are exact integers of at most 128 * 128 * 128 < 2^22, and they start at the integer whose bits are the
 // float 1.5 * 2^23, so that their own bits are that float plus the sum. From there on it is 32-bit floating
-// arithmetic: scales are never rounded and multiply each group's sum. A block of x that holds an infinity or
-// a NaN makes its row NaN. What bounds it now is instructions, 180 for 16 x 128 weights in groups of 32: experts
+// arithmetic: scales are never rounded and multiply each group's sum. What bounds it now is instructions, 180 for 16 x 128 weights in groups of 32: experts
 // at 8 tokens take 87 us, without the copies 80, without the products 68, against 45 for their bytes.
 #include "ffn_internal.h"
 
 #include <cmath>
+#include <cstring>
 #include <type_traits>
 
 namespace cernels {
@@ -64,6 +72,18 @@ __device__ __forceinline__ void mma_bytes(int4& d, const int4& c, uint32_t a0, u
 
 constexpr int kFloatBias = 0x4b400000;       // the bits of 1.5 * 2^23: adding n < 2^22 to them adds n to the float
 constexpr float kFloatBiasValue = 12582912.0f;
+
+// Codes 2 i and 2 i + 1 of a word of eight as bf16 values q - 8: 0x4300 | q is 128 + q.
+__device__ __forceinline__ uint32_t bf16_codes(uint32_t word, int i) {
+  const uint32_t t = word >> 8 * i, biased = (t & 0xfu) | (t << 12 & 0xf0000u) | 0x43004300u;
+  const __nv_bfloat162 v = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&biased), __float2bfloat162_rn(136.0f));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Bytes of a word that are not zero, as their top bits.
+__device__ __forceinline__ uint32_t nonzero_bytes(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w) & 0x80808080u;
+}
 
 // Two 32-bit values at once (FFMA2 and the like: half the instructions of the scalar forms).
 struct Two {
@@ -169,7 +189,7 @@ __host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int tile_c
   off += static_cast<size_t>(warps) * kDepth * slot;
   s.part = off;
   off += static_cast<size_t>(part_buffers(warps)) * warps * tile_cols * 16 * 4;
-  s.units = off;  // per column and block: 2^e / 16
+  s.units = off;  // per column and block: 2^e / 16, or 0 for a mixed block
   off += (static_cast<size_t>(blocks) * cols * 4 + 15) / 16 * 16;
   s.x = off;
   off += static_cast<size_t>(cols) * x_row_bytes(padded_k);
@@ -192,7 +212,7 @@ __host__ __device__ inline SkinnySmem carve_smem(int warps, int slot, int tile_c
   off += n * 2;
   s.order = off;
   off += n * 2;
-  s.total = off + 16;
+  s.total = off + 16;  // number of items, mark of the last item with a mixed block
   return s;
 }
 
@@ -298,6 +318,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   float* part = reinterpret_cast<float*>(smem + lay.part);
   const int blocks = padded_k / 128;
   float* units_of_x = reinterpret_cast<float*>(smem + lay.units);  // [column][block]
+  int* mixed_mark = reinterpret_cast<int*>(smem + lay.total - 12);
   uint8_t* xs = smem + lay.x;
   const Item* items = reinterpret_cast<const Item*>(smem + lay.items);
   const uint16_t* order = reinterpret_cast<const uint16_t*>(smem + lay.order);
@@ -430,25 +451,55 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   constexpr int kBatch = 8;
   const int row_chunks = padded_k / 256;
   const unsigned inverse_chunks = (1u << 20) / (row_chunks ? row_chunks : 1) + 1;  // chunk / row_chunks, exact for up to 16 * 128
+  auto load_piece = [&](const Item& it, unsigned chunk) {
+    const int c = static_cast<int>(chunk * inverse_chunks >> 20);
+    const int k = (static_cast<int>(chunk) - c * row_chunks) * 256 + lane * 8;
+    int row = it.first + c;
+    if (routed) {
+      row = order[row];
+      if (!a.x_by_pair) row /= a.topk;
+    }
+    return k < a.k ? *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(row) * a.x_stride + k) : make_uint4(0, 0, 0, 0);
+  };
   auto fetch_x = [&](const Item& it, int first_chunk, uint4 (&v)[kBatch]) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const unsigned chunk = first_chunk + b * kWarps;
       v[b] = make_uint4(0, 0, 0, 0);
-      if (static_cast<int>(chunk) < it.count * row_chunks) {
-        const int c = static_cast<int>(chunk * inverse_chunks >> 20);
-        const int k = (static_cast<int>(chunk) - c * row_chunks) * 256 + lane * 8;
-        int row = it.first + c;
-        if (routed) {
-          row = order[row];
-          if (!a.x_by_pair) row /= a.topk;
-        }
-        if (k < a.k) v[b] = *reinterpret_cast<const uint4*>(a.x + static_cast<size_t>(row) * a.x_stride + k);
+      if (static_cast<int>(chunk) < it.count * row_chunks) v[b] = load_piece(it, chunk);
+    }
+  };
+  // Gives the mixed blocks of a batch the unit 0, and the item its mark.
+  auto mark_mixed = [&](const Item& it, int mark, int first_chunk) {
+#pragma unroll 1
+    for (int chunk = first_chunk; chunk < min(first_chunk + kBatch * kWarps, it.count * row_chunks); chunk += kWarps) {
+      const uint4 v = load_piece(it, chunk);
+      const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) top = max(top, max(words[j] << 16 & 0x7fff0000u, words[j] & 0x7fff0000u));
+#pragma unroll
+      for (unsigned d = 8; d > 0; d /= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+      const int least = max(static_cast<int>(top >> 23) - 13, 5) + 7;  // exponent of 128 units
+      int votes = 0;  // of the nonzero values: +1 small, -1 large
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t size = j & 1 ? words[j >> 1] & 0x7fff0000u : words[j >> 1] << 16 & 0x7fff0000u;
+        votes += size == 0 ? 0 : static_cast<int>(size >> 23) < least ? 1 : -1;
+      }
+#pragma unroll
+      for (unsigned d = 8; d > 0; d /= 2) votes += __shfl_xor_sync(0xffffffffu, votes, d);
+      if ((votes > 0 || top >= 0x7f800000u) && lane % 16 == 0) {
+        const int c = chunk / row_chunks;
+        units_of_x[c * blocks + (chunk - c * row_chunks) * 2 + lane / 16] = 0.f;
+        *mixed_mark = mark;
       }
     }
   };
-  auto store_x = [&](const Item& it, int first_chunk, const uint4 (&v)[kBatch]) {
+  auto store_x = [&](const Item& it, int mark, int first_chunk, const uint4 (&v)[kBatch]) {
     if constexpr (kFmt != 0) {
+      uint32_t large[kBatch / 4] = {0x04040404u, 0x04040404u};  // a byte for each chunk, 64 in all where there is none
+      uint32_t special = 0;
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
         const unsigned chunk = first_chunk + b * kWarps;
@@ -474,16 +525,27 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
           return __byte_perm(__byte_perm(n[odd] + add, n[odd + 2] + add, selector),
                              __byte_perm(n[odd + 4] + add, n[odd + 6] + add, selector), 0x5410);
         };
-        if (k8 % 16 == 0)
-          units_of_x[c * blocks + k8 / 16] =
-              __uint_as_float(top >= 0x7f800000u ? 0x7fc00000u : static_cast<uint32_t>(unit_exp - 4) << 23);
+        const uint4 split_x = make_uint4(bytes(0x51, 0, 128), bytes(0x51, 1, 128), bytes(0x40, 0, 0), bytes(0x40, 1, 0));
+        // values of 128 units or more, by their high byte; past the row's end half of the places count
+        const uint32_t found = static_cast<int>(k8) * 8 < a.k ? __popc(nonzero_bytes(split_x.x) | nonzero_bytes(split_x.y) >> 1) : 4;
+        large[b / 4] += (found - 4) << 8 * (b % 4);
+        special = max(special, top);
+        if (k8 % 16 == 0) units_of_x[c * blocks + k8 / 16] = __uint_as_float(static_cast<uint32_t>(unit_exp - 4) << 23);
         constexpr unsigned kPer = kFmt / 8;  // pieces per group
         const unsigned in = k8 % kPer;
         // group | lane of the quad | word  ->  group | word | lane
         const unsigned at = k8 - in + (in % F::kWords) * 4 + in / F::kWords;
-        *reinterpret_cast<uint4*>(xs + static_cast<size_t>(c) * x_bytes + at * 16) =
-            make_uint4(bytes(0x51, 0, 128), bytes(0x51, 1, 128), bytes(0x40, 0, 0), bytes(0x40, 1, 0));
+        *reinterpret_cast<uint4*>(xs + static_cast<size_t>(c) * x_bytes + at * 16) = split_x;
       }
+#pragma unroll
+      for (unsigned d = 8; d > 0; d /= 2)
+#pragma unroll
+        for (int j = 0; j < kBatch / 4; ++j) large[j] += __shfl_xor_sync(0xffffffffu, large[j], d);
+      // a count under 64 in any block: bits 6 and 7 of its byte are clear
+      uint32_t enough = 0x40404040u;
+#pragma unroll
+      for (int j = 0; j < kBatch / 4; ++j) enough &= large[j] | large[j] >> 1;
+      if (__any_sync(0xffffffffu, enough != 0x40404040u || special >= 0x7f800000u)) mark_mixed(it, mark, first_chunk);
     }
   };
   auto copy_x = [&](const Item& it) {  // bf16
@@ -496,7 +558,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     }
     commit_copies();
   };
-  auto load_x = [&](const Item& it, int first_chunk) {
+  auto load_x = [&](const Item& it, int mark, int first_chunk) {
     if constexpr (kFmt == 0) {
       copy_x(it);
       wait_copies<0>();
@@ -504,7 +566,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
       for (int chunk = first_chunk; chunk < it.count * row_chunks; chunk += kWarps * kBatch) {
         uint4 v[kBatch];
         fetch_x(it, chunk, v);
-        store_x(it, chunk, v);
+        store_x(it, mark, chunk, v);
       }
     }
   };
@@ -527,13 +589,13 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     if constexpr (kFmt != 0)
       fetch_x(item, warp, first_x);
     else
-      load_x(item, 0);
+      load_x(item, 0, 0);
   } else if constexpr (kFmt == 0) {
     wait_copies<kDepth>();
   }
   if constexpr (kFmt != 0) {
-    store_x(item, warp, first_x);
-    load_x(item, warp + kWarps * kBatch);
+    store_x(item, item_index + 1, warp, first_x);
+    load_x(item, item_index + 1, warp + kWarps * kBatch);
   }
   __syncthreads();
   // Columns past the item's last read its last one again: their sums are never used.
@@ -550,6 +612,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     }
   };
   point_x();
+  // What the word holds before the first mark may look like one: then no block's unit is 0 all the same.
+  bool any_mixed = kFmt != 0 && *mixed_mark == item_index + 1;
   // start of every group's sums; opaque, so that it stays in registers
   int4 start;
   asm volatile("mov.b32 %0, %4;\n\tmov.b32 %1, %4;\n\tmov.b32 %2, %4;\n\tmov.b32 %3, %4;"
@@ -577,6 +641,82 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     }
   };
   point_scales();
+  // The products of the unit's mixed blocks in this warp's steps, with codes, scales and x from global memory (L2 has
+  // them). The sums of integers left these blocks' columns out: their units are 0.
+  auto add_mixed = [&] {
+    if constexpr (kFmt != 0) {
+      const int base = (unit * tiles_at_once + rt) * kOut;
+      const size_t e = routed ? item.expert : 0;
+      const size_t ra = min(base + g, a.rows - 1), rb = kGateUp ? ra : min(base + g + 8, a.rows - 1);
+      const uint8_t* wa = a.w0 + e * a.w_expert + ra * row_bytes;
+      const uint8_t* wb = (kGateUp ? a.w1 : a.w0) + e * a.w_expert + rb * row_bytes;
+      const uint16_t* fa = a.s0 + e * a.s_expert + ra * row_groups;
+      const uint16_t* fb = (kGateUp ? a.s1 : a.s0) + e * a.s_expert + rb * row_groups;
+      const __nv_bfloat16* x_row[NT];  // of the column whose values this lane gives the mma (packed: its even columns)
+      unsigned column[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        column[n] = kPacked ? (g & 1 ? 31 : g >> 1) : n * 8 + g;
+        size_t row = item.first + min(static_cast<int>(column[n]), item.count - 1);
+        if (routed) {
+          row = order[row];
+          if (!a.x_by_pair) row /= a.topk;
+        }
+        x_row[n] = a.x + row * a.x_stride;
+      }
+#pragma unroll 1
+      for (int block = kw * kParts; block < steps * kParts; block += block % kParts == kParts - 1 ? (a.k_warps - 1) * kParts + 1 : 1) {
+        const unsigned mixed = __ballot_sync(0xffffffffu, lane < item.count && units_of_x[min(lane, item.count - 1) * blocks + block] == 0.f);
+        if (mixed == 0) continue;
+        // lane q's words of a group: kWords in a row; groups past the row's end are empty
+        uint32_t ca[F::kGroups * F::kWords], cb[F::kGroups * F::kWords];
+        float scale_a[F::kGroups], scale_b[F::kGroups];
+        const int group = block * F::kGroups, left = row_groups - group;
+#pragma unroll
+        for (int s = 0; s < F::kGroups; ++s) {
+          using Words = std::conditional_t<F::kWords == 4, uint4, std::conditional_t<F::kWords == 2, uint2, uint32_t>>;
+          Words u{}, v{};
+          scale_a[s] = scale_b[s] = 0.f;
+          if (s < left) {
+            u = reinterpret_cast<const Words*>(wa + (group + s) * (kFmt / 2))[q];
+            v = reinterpret_cast<const Words*>(wb + (group + s) * (kFmt / 2))[q];
+            scale_a[s] = __uint_as_float(static_cast<uint32_t>(fa[group + s]) << 16);
+            scale_b[s] = __uint_as_float(static_cast<uint32_t>(fb[group + s]) << 16);
+          }
+          memcpy(ca + s * F::kWords, &u, sizeof(u));
+          memcpy(cb + s * F::kWords, &v, sizeof(v));
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const bool mine = mixed >> column[n] & 1;
+          uint4 x8[F::kGroups * F::kWords];
+#pragma unroll
+          for (int j = 0; j < F::kGroups * F::kWords; ++j) {
+            const int s = j / F::kWords, piece = (group + s) * (kFmt / 8) + q * F::kWords + j % F::kWords;  // of eight values
+            x8[j] = make_uint4(0, 0, 0, 0);
+            if (mine && s < left) x8[j] = *reinterpret_cast<const uint4*>(x_row[n] + piece * 8);
+          }
+#pragma unroll
+          for (int s = 0; s < F::kGroups; ++s) {
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < F::kWords; ++w) {
+              const int j = s * F::kWords + w;
+              mma_bf16(sum, bf16_codes(ca[j], 0), bf16_codes(cb[j], 0), bf16_codes(ca[j], 1), bf16_codes(cb[j], 1), x8[j].x, x8[j].y);
+              mma_bf16(sum, bf16_codes(ca[j], 2), bf16_codes(cb[j], 2), bf16_codes(ca[j], 3), bf16_codes(cb[j], 3), x8[j].z, x8[j].w);
+            }
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (kPacked ? j == 0 && mixed >> q & 1 : mixed >> (n * 8 + 2 * q + j) & 1) {
+                acc[n][j] = fmaf(scale_a[s], sum[j], acc[n][j]);
+                acc[n][j + 2] = fmaf(scale_b[s], sum[j + 2], acc[n][j + 2]);
+              }
+            }
+          }
+        }
+      }
+    }
+  };
   while (true) {
     const int step = i * a.k_warps + kw;
     wait_copies<kDepth - 1>();
@@ -696,6 +836,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     if (++i == per_warp) {
       // ---- end of the unit: add the sums of each tile's warps (in warp order) and write
       i = 0;
+      if (any_mixed) add_mixed();
       float* mine = part + ((buffer * kWarps + warp) * kCols + (kPacked ? q : 2 * q)) * 16 + g;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -738,9 +879,10 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
       if (++unit == per_item) {  // the next item's x rows; every warp has used the old ones
         unit = 0;
         item = item_of(++item_index);
-        load_x(item, warp);
+        load_x(item, item_index + 1, warp);
         __syncthreads();
         point_x();
+        any_mixed = kFmt != 0 && *mixed_mark == item_index + 1;
       }
       point_scales();
     }

@@ -5,6 +5,10 @@ half) and K / G bf16 scales, G 32, 64 or 128::
 
     W[n, k] = (q[n, k] - 8) * scale[n, k // G]
 
+Weights are never rounded and sums are in 32 bits. A block of 128 values of x is taken as 14 bits and a sign below its
+largest value if at least half of its nonzero values are exact that way (none is then off by more than 2^-8 of the
+block's median); else, and with an infinity or a NaN in it, it is multiplied exactly in bf16.
+
 ``linear_w4`` is a linear layer for a few rows; ``moe_experts_decode_w4`` is the routed experts'
 decode call (``*_moe_experts_decode``) on such weights, a quarter of the bytes that bound it;
 ``quantize_w4`` makes the codes and scales from bf16 weights. The first two are

@@ -286,7 +286,9 @@ int cernels_gated_ffn_backward(const cernels_ffn_shape* shape, const void* x, in
  * counterpart in the reference, whose weights are bf16). A weight row of K values is K / 2 bytes,
  * two codes a byte with the even position in the low half, and K / group bf16 scales:
  *   W[n, k] = (q[n, k] - 8) * scale[n, k / group],   group 32, 64 or 128, K a multiple of it.
- * Sums are in 32 bits, weights are never rounded. x, codes and the experts' scales and outputs are 16-byte
+ * Sums are in 32 bits, weights are never rounded. A block of 128 values of x is taken as 14 bits and a sign
+ * below its largest value if at least half of its nonzero values are exact that way (none is then off by more than
+ * 2^-8 of the block's median); else, and with an infinity or a NaN in it, it is multiplied exactly in bf16. x, codes and the experts' scales and outputs are 16-byte
  * aligned, a linear layer's scales 4-byte. */
 
 /* out[t, n] = sum_k x[t, k] W[n, k]: x [T, K] bf16 (row stride x_stride, a multiple of 8), out
