@@ -96,12 +96,26 @@ int sm_count_cached() {
   return counts[dev];
 }
 
+// Whether this host thread has a current context.
+bool has_context() {
+  static const auto current = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    return cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                   q == cudaDriverEntryPointSuccess
+               ? reinterpret_cast<CUresult (*)(CUcontext*)>(p)
+               : nullptr;
+  }();
+  CUcontext context = nullptr;
+  return current && current(&context) == CUDA_SUCCESS && context != nullptr;
+}
+
 int check_device() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return CERNELS_E_CUDA;
-  // Binds the device's context to this host thread: the driver call that encodes TMA maps needs
-  // one, and a thread whose first CUDA call this is (autograd's) has none yet.
-  if (cudaSetDevice(dev) != cudaSuccess) return CERNELS_E_CUDA;
+  // The driver call that encodes TMA maps needs a context, and a thread whose first CUDA call this is
+  // (autograd's) has none yet: it gets the device's. One that the caller has made current stays.
+  if (!has_context() && cudaSetDevice(dev) != cudaSuccess) return CERNELS_E_CUDA;
   static std::atomic<signed char> known[64];  // 0 not asked yet, 1 sm_100, -1 another device
   signed char state = dev < 64 ? known[dev].load(std::memory_order_relaxed) : 0;
   if (state == 0) {
