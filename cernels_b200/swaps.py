@@ -11,6 +11,7 @@ SWAPS maps a model name to (apply(model, variant), variants), stock first.
 
 from __future__ import annotations
 
+import functools
 from typing import Callable
 
 import torch
@@ -106,23 +107,33 @@ def _linear_family(cls_name: str):
     return apply
 
 
+def _mlp_forward(mlp, x):
+    from .registry import gated_ffn
+
+    return gated_ffn.kernel(x, mlp)
+
+
 def swap_mlps(model: torch.nn.Module, cls_name: str, custom: bool) -> int:
     """Sets (or restores) the forward of every `cls_name` instance, a dense gated MLP (gate_proj, up_proj,
-    down_proj), to the gated feed-forward operator, which is differentiable. Returns the number of
-    modules touched; raises when the model has none."""
+    down_proj), to the gated feed-forward operator, which is differentiable. A forward that something else has set on an
+    instance is neither replaced (that raises, and leaves the model as it was) nor taken away. Returns the number of
+    modules of the class; raises when the model has none."""
     from .registry import gated_ffn
 
     mods = [m for m in model.modules() if type(m).__name__ == cls_name]
     if not mods:
         raise RuntimeError(f"no {cls_name} modules found — wrong model for this swap")
+    ours = [getattr(vars(m).get("forward"), "func", None) is _mlp_forward for m in mods]
     if custom:  # all of them or none
-        for mod in mods:
+        for mod, mine in zip(mods, ours):
+            if "forward" in vars(mod) and not mine:
+                raise RuntimeError(f"a {cls_name} has a forward of its own, which this swap would replace")
             gated_ffn.check_module(mod)
-    for mod in mods:
-        if "forward" in vars(mod):
+    for mod, mine in zip(mods, ours):
+        if mine:
             del mod.forward
         if custom:
-            mod.forward = lambda x, _m=mod: gated_ffn.kernel(x, _m)
+            mod.forward = functools.partial(_mlp_forward, mod)
     return len(mods)
 
 

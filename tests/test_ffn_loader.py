@@ -112,3 +112,24 @@ def test_the_transformers_modules_are_taken():
     small = dict(hidden_size=64, intermediate_size=96, hidden_act="silu")
     for mlp in (Deepseek(transformers.DeepseekV2Config(**small)), Qwen(transformers.Qwen3NextConfig(**small), 96)):
         gated_ffn.check_module(mlp)
+
+
+def test_a_forward_that_something_else_set_is_kept():
+    """Wrappers that move weights or time calls set an instance's forward: the swap neither replaces nor removes it."""
+    apply = swaps.SWAPS["deepseek_v2_mlp"][0]
+    m = torch.nn.ModuleList([DeepseekV2MLP(), DeepseekV2MLP()])
+    plain = m[1].forward
+
+    def timed(x):
+        return plain(x)
+
+    m[1].forward = timed
+    with pytest.raises(RuntimeError, match="forward of its own"):
+        apply(m, "custom")
+    assert "forward" not in vars(m[0]) and m[1].forward is timed
+    assert apply(m, "stock") == 2 and m[1].forward is timed
+    del m[1].forward
+    assert apply(m, "custom") == 2 and apply(m, "custom") == 2  # its own it does replace
+    m[0].forward = timed  # set over the swap's
+    assert apply(m, "stock") == 2
+    assert m[0].forward is timed and "forward" not in vars(m[1])
