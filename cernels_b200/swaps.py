@@ -19,14 +19,13 @@ import torch
 DECODE_MAX_TOKENS = 4  # at or below this many tokens the decode entry point handles the op
 
 
-def _experts_fwd(mod, kernel: Callable | None, decode_kernel: Callable | None):
-    def fwd(h, idx, w, _m=mod):
-        op = decode_kernel if h.size(0) <= DECODE_MAX_TOKENS else kernel
-        if op is None:  # this shape's entry point is not enabled in this variant
-            return type(_m).forward(_m, h, idx, w)
-        return op(h, idx, w, _m)
-
-    return fwd
+# Forwards are partial objects of the module: a copy of a swapped model (copy.deepcopy) gets ones of its own modules,
+# where a closure would go on computing with the original's.
+def _experts_forward(mod, kernel: Callable | None, decode_kernel: Callable | None, h, idx, w):
+    op = decode_kernel if h.size(0) <= DECODE_MAX_TOKENS else kernel
+    if op is None:  # this shape's entry point is not enabled in this variant
+        return type(mod).forward(mod, h, idx, w)
+    return op(h, idx, w, mod)
 
 
 def swap_experts(model: torch.nn.Module, cls_name: str, kernel: Callable | None,
@@ -41,7 +40,7 @@ def swap_experts(model: torch.nn.Module, cls_name: str, kernel: Callable | None,
         if "forward" in vars(mod):
             del mod.forward
         if kernel is not None or decode_kernel is not None:
-            mod.forward = _experts_fwd(mod, kernel, decode_kernel)
+            mod.forward = functools.partial(_experts_forward, mod, kernel, decode_kernel)
     if not n:
         raise RuntimeError(f"no {cls_name} modules found — wrong model for this swap")
     return n

@@ -1,11 +1,13 @@
 """Which modules the gated block's loader and swap take: those that compute what the operator computes."""
 
+import copy
+
 import pytest
 import torch
 
 from cernels_b200 import swaps
-from cernels_b200.registry import gated_ffn
-from tests.test_ffn_modules import DeepseekV2MLP
+from cernels_b200.registry import gated_ffn, moe_experts_w4
+from tests.test_ffn_modules import DeepseekV2Experts, DeepseekV2MLP
 
 
 class Adapter(torch.nn.Module):  # a low-rank adapter that shows its base layer's weight and bias
@@ -133,3 +135,21 @@ def test_a_forward_that_something_else_set_is_kept():
     m[0].forward = timed  # set over the swap's
     assert apply(m, "stock") == 2
     assert m[0].forward is timed and "forward" not in vars(m[1])
+
+
+def test_copies_of_swapped_models_compute_with_their_own_weights(monkeypatch):
+    seen = []
+    monkeypatch.setattr(gated_ffn, "kernel", lambda x, mlp: seen.append(mlp))
+    monkeypatch.setattr(moe_experts_w4, "decode_kernel", lambda x, idx, w, experts: seen.append(experts))
+    m = torch.nn.ModuleList([DeepseekV2MLP(), DeepseekV2Experts()])
+    swaps.SWAPS["deepseek_v2_mlp"][0](m, "custom")
+    swaps.SWAPS["deepseek_v2"][0](m, "custom_w4")
+    c = copy.deepcopy(m)
+    x, idx, w = torch.zeros(2, 64), torch.zeros(2, 2), torch.zeros(2, 2)
+    for mod, args in zip(c, ((x,), (x, idx, w))):
+        mod(*args)
+    assert seen[0] is c[0] and seen[1] is c[1]
+    assert c[1]._cernels_w4[0] is not m[1]._cernels_w4[0]
+    for apply in (swaps.SWAPS["deepseek_v2_mlp"][0], swaps.SWAPS["deepseek_v2"][0]):
+        assert apply(c, "stock") == 1
+    assert not any("forward" in vars(mod) for mod in c) and all("forward" in vars(mod) for mod in m)
