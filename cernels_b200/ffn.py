@@ -241,14 +241,18 @@ def _meta_grads(dout, x, gate_proj, up_proj, down_proj, act, saved, needs):
     return [t.new_empty(t.shape) for t, need in zip((x, gate_proj, up_proj, down_proj), needs) if need]
 
 
-def status(device: torch.device | int | None = None) -> int:
-    """0, or the code of a bounded wait that gave up in one of these kernels on `device` since the
-    last call (the results since then are not to be used). Synchronises the current stream."""
+def status(device: torch.device | str | int | None = None) -> int:
+    """0, or the code of a bounded wait that gave up in one of these kernels on `device` (default: the current one) since
+    the last call, whoever made it; the results since then are not to be used. Synchronises the current stream."""
     code = ctypes.c_int(0)
-    dev = torch.device("cuda", torch.cuda.current_device() if device is None else torch.device("cuda", device).index
-                       if isinstance(device, int) else device.index)
-    with torch.cuda.device(dev):
-        _lib.check(_lib.load().cernels_ffn_status(ctypes.byref(code), torch.cuda.current_stream(dev).cuda_stream),
+    index = device if isinstance(device, int) else None
+    if device is not None and index is None:
+        dev = torch.device(device)
+        _check(dev.type == "cuda", f"no such word on {dev}")
+        index = dev.index
+    index = torch.cuda.current_device() if index is None else index
+    with torch.cuda.device(index):
+        _lib.check(_lib.load().cernels_ffn_status(ctypes.byref(code), torch.cuda.current_stream(index).cuda_stream),
                    "cernels_ffn_status")
     return code.value
 

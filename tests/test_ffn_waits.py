@@ -1,12 +1,17 @@
 """Tile products whose waits give up (a hang that should never be): what is in flight then has to end
 before the CTAs of a pair leave. The rule for it (csrc/pair_drain.h) runs here on the CPU, against a model of
-the stages' barriers, for every way in which the two CTAs can have stopped."""
+the stages' barriers, for every way in which the two CTAs can have stopped. And the word that tells of it
+(``ffn.status``), over a stand-in for the library."""
 
+import contextlib
 import shutil
 import subprocess
+import types
 
 import pytest
+import torch
 
+from cernels_b200 import ffn
 from cernels_b200.build import CSRC
 
 MODEL = r"""
@@ -82,3 +87,38 @@ def test_every_load_in_flight_is_waited_for(tmp_path):
     subprocess.run(["g++", "-std=c++17", "-O2", "-I", str(CSRC), str(source), "-o", str(program)], check=True)
     run = subprocess.run([str(program)], capture_output=True, text=True, timeout=120)
     assert run.returncode == 0, run.stdout
+
+
+@pytest.mark.parametrize("device,index", [(None, 3), (0, 0), (2, 2), (torch.device("cuda"), 3), (torch.device("cuda", 0), 0),
+                                          (torch.device("cuda:5"), 5), ("cuda", 3), ("cuda:1", 1)])
+def test_status_reads_the_word_of_the_device_that_is_asked_for(monkeypatch, device, index):
+    words, current, calls = {index: 2}, [3], []
+
+    @contextlib.contextmanager
+    def on(d):
+        before, current[0] = current[0], d
+        yield
+        current[0] = before
+
+    def read(code, stream):  # as the C entry: reads and clears the current device's word
+        calls.append((current[0], stream))
+        code._obj.value = words.pop(current[0], 0)
+        return 0
+
+    monkeypatch.setattr(ffn._lib, "load", lambda: types.SimpleNamespace(cernels_ffn_status=read))
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", on)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: types.SimpleNamespace(cuda_stream=100 + d))
+    assert ffn.status(device) == 2 and ffn.status(device) == 0
+    assert calls == [(index, 100 + index)] * 2 and current == [3]
+
+
+def test_status_refusals(monkeypatch):
+    with pytest.raises(RuntimeError, match="cpu"):
+        ffn.status("cpu")
+    monkeypatch.setattr(ffn._lib, "load", lambda: types.SimpleNamespace(
+        cernels_ffn_status=lambda code, stream: 4, cernels_error_string=lambda code: b"CUDA error"))
+    monkeypatch.setattr(torch.cuda, "device", contextlib.nullcontext)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda d: types.SimpleNamespace(cuda_stream=0))
+    with pytest.raises(RuntimeError, match="cernels_ffn_status"):  # an error of the call is not a status
+        ffn.status(0)
