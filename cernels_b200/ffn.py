@@ -30,6 +30,13 @@ def rows_ok(x: torch.Tensor) -> bool:
     return x.stride(1) == 1 and (x.shape[0] <= 1 or (x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0))
 
 
+def readable(x: torch.Tensor) -> torch.Tensor:
+    """x, or a copy of it where the kernels cannot read its rows in place: for loaders, whose modules take any x."""
+    if rows_ok(x) and (traced(x) or x.data_ptr() % 16 == 0):
+        return x
+    return x.clone(memory_format=torch.contiguous_format)
+
+
 def int32_sizes(*sizes: int) -> None:
     """Refuses sizes that the C ABI's 32-bit fields would wrap."""
     _check(max(sizes) < 1 << 31, "sizes must be below 2^31")

@@ -9,7 +9,7 @@ differentiable, in x and the module's weights.
 
 import torch
 
-from ..ffn import gated_ffn, rows_ok
+from ..ffn import gated_ffn, readable
 
 
 _PROJECTIONS = ("gate_proj", "up_proj", "down_proj")
@@ -51,6 +51,6 @@ def check_module(mlp) -> None:
 
 def kernel(x, mlp):
     check_module(mlp)
-    xf = x.reshape(-1, x.shape[-1])
-    y = gated_ffn(xf if rows_ok(xf) else xf.contiguous(), mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight)
+    xf = readable(x.reshape(-1, x.shape[-1]))
+    y = gated_ffn(xf, mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight)
     return y.reshape(x.shape)

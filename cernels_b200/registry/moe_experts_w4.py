@@ -11,6 +11,7 @@ are made when ``prepare`` is called and not looked after: call it again when the
 import torch
 
 from .. import w4
+from ..ffn import readable
 from ._common import routing_tensors
 
 _SLOT = "_cernels_w4"
@@ -49,4 +50,4 @@ def decode_kernel(x, top_k_index, top_k_weights, experts):
         raise RuntimeError("no 4-bit weights on this module: call moe_experts_w4.prepare(experts) first")
     with torch.no_grad():
         idx, w = routing_tensors(top_k_index, top_k_weights)
-        return w4.moe_experts_decode_w4(x.contiguous(), *copies, idx, w, int(top_k_index.size(1)))
+        return w4.moe_experts_decode_w4(readable(x.contiguous()), *copies, idx, w, int(top_k_index.size(1)))

@@ -5,7 +5,7 @@ import copy
 import pytest
 import torch
 
-from cernels_b200 import swaps
+from cernels_b200 import swaps, w4
 from cernels_b200.registry import gated_ffn, moe_experts_w4
 from tests.test_ffn_modules import DeepseekV2Experts, DeepseekV2MLP
 
@@ -153,3 +153,50 @@ def test_copies_of_swapped_models_compute_with_their_own_weights(monkeypatch):
     for apply in (swaps.SWAPS["deepseek_v2_mlp"][0], swaps.SWAPS["deepseek_v2"][0]):
         assert apply(c, "stock") == 1
     assert not any("forward" in vars(mod) for mod in c) and all("forward" in vars(mod) for mod in m)
+
+
+def odd_view(x):
+    """The same values 2 bytes off a 16-byte boundary."""
+    wide = torch.zeros(x.numel() + 9, dtype=x.dtype, device=x.device)
+    off = (2 - wide.data_ptr()) % 16 // 2
+    view = wide[off:off + x.numel()].view(x.shape)
+    view.copy_(x)
+    assert view.data_ptr() % 16 == 2
+    return view
+
+
+@pytest.mark.parametrize("make", [lambda x: x, odd_view, lambda x: x.transpose(0, 1).contiguous().transpose(0, 1),
+                                  lambda x: x[:1].expand(3, 2, 64), lambda x: odd_view(x)[:, 1:]],
+                         ids=["plain", "odd", "transposed", "expanded", "odd slice"])
+def test_loaders_hand_over_rows_that_the_kernels_can_read(monkeypatch, make):
+    x = make(torch.randn(3, 2, 64).to(torch.bfloat16))
+    got = []
+
+    def take(rows, *rest):
+        got.append(rows)
+        return rows
+
+    monkeypatch.setattr(gated_ffn, "gated_ffn", take)
+    monkeypatch.setattr(w4, "moe_experts_decode_w4", take)
+    assert torch.equal(gated_ffn.kernel(x, DeepseekV2MLP()), x)
+    e = DeepseekV2Experts()
+    moe_experts_w4.prepare(e)
+    flat = x[:, 0]
+    moe_experts_w4.decode_kernel(flat, torch.zeros(3, 2), torch.zeros(3, 2), e)
+    assert torch.equal(got[1], flat) and got[1].is_contiguous()
+    assert all(t.data_ptr() % 16 == 0 and t.stride(1) == 1 for t in got)
+
+
+@pytest.mark.gpu
+def test_a_misaligned_x_through_the_swapped_modules():
+    torch.manual_seed(3)
+    m = torch.nn.ModuleList([DeepseekV2MLP(device="cuda"), DeepseekV2Experts(device="cuda")])
+    swaps.SWAPS["deepseek_v2_mlp"][0](m, "custom")
+    swaps.SWAPS["deepseek_v2"][0](m, "custom_w4")
+    x = torch.randn(3, 64, device="cuda").to(torch.bfloat16)
+    w, idx = torch.rand(3, 4, device="cuda").topk(2, -1)
+    with torch.no_grad():
+        assert torch.equal(m[0](odd_view(x)), m[0](x)) and torch.equal(m[1](odd_view(x), idx, w), m[1](x, idx, w))
+    a, b = x.clone().requires_grad_(), odd_view(x).requires_grad_()
+    dy = torch.randn_like(x)
+    assert torch.equal(torch.autograd.grad(m[0](a), a, dy)[0], torch.autograd.grad(m[0](b), b, dy)[0])
