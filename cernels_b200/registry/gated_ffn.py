@@ -4,7 +4,8 @@ down_proj and SiLU), which the reference runs as they are
 (src/kops/registry/qwen3_next_moe_experts.py:31-44).
 
 ``kernel(x, mlp)`` takes hidden states [..., H] and the module. Unlike the experts' loaders it is
-differentiable, in x and the module's weights.
+differentiable, in x and the module's weights; under ``torch.autocast`` to bf16 x and weights of other
+types are cast to it, as they are for the module.
 """
 
 import torch
@@ -51,6 +52,9 @@ def check_module(mlp) -> None:
 
 def kernel(x, mlp):
     check_module(mlp)
-    xf = readable(x.reshape(-1, x.shape[-1]))
-    y = gated_ffn(xf, mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight)
-    return y.reshape(x.shape)
+    t = x, mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight
+    if torch.is_autocast_enabled("cuda") and torch.get_autocast_dtype("cuda") is torch.bfloat16:
+        x, *w = (v.to(torch.bfloat16) for v in t)  # as autocast does for the module's linear layers
+    else:
+        x, *w = t
+    return gated_ffn(readable(x.reshape(-1, x.shape[-1])), *w).reshape(x.shape)

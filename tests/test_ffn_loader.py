@@ -7,6 +7,7 @@ import torch
 
 from cernels_b200 import swaps, w4
 from cernels_b200.registry import gated_ffn, moe_experts_w4
+from tests import ffn_reference as R
 from tests.test_ffn_modules import DeepseekV2Experts, DeepseekV2MLP
 
 
@@ -200,3 +201,28 @@ def test_a_misaligned_x_through_the_swapped_modules():
     a, b = x.clone().requires_grad_(), odd_view(x).requires_grad_()
     dy = torch.randn_like(x)
     assert torch.equal(torch.autograd.grad(m[0](a), a, dy)[0], torch.autograd.grad(m[0](b), b, dy)[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.float32, torch.bfloat16])
+def test_autocast_casts_as_the_module_does(kind):
+    """32-bit weights in training: the gradients of the cast weights, in 32 bits."""
+    torch.manual_seed(4)
+    mlp = DeepseekV2MLP(device="cuda").float()
+    model = torch.nn.ModuleList([mlp])
+    x = torch.randn(40, 64, device="cuda", dtype=kind).requires_grad_()
+    dy = torch.randn(40, 64, device="cuda").to(torch.bfloat16)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        stock = mlp(x)
+        swaps.SWAPS["deepseek_v2_mlp"][0](model, "custom")
+        y = mlp(x)
+    assert y.dtype == stock.dtype == torch.bfloat16
+    weights = [mlp.gate_proj.weight, mlp.up_proj.weight, mlp.down_proj.weight]
+    cast = [v.detach().to(torch.bfloat16) for v in (x, *weights)]
+    want, bound, state = R.forward(*cast)
+    R.assert_within("y", y.detach(), want, bound)
+    for t, g, (w, b) in zip((x, *weights), torch.autograd.grad(y, (x, *weights), dy), R.backward(state, dy)):
+        assert g.dtype == t.dtype
+        R.assert_within("gradient", g, w, b)
+    with pytest.raises(RuntimeError, match="bf16"):  # no autocast, no cast
+        mlp(x)
