@@ -114,13 +114,14 @@ _PLAIN = frozenset((torch.Tensor, torch.nn.Parameter))
 _compiling = torch.compiler.is_compiling
 _modes = torch._C._len_torch_dispatch_stack
 _transform = torch._C._functorch.peek_interpreter_stack
+_jit = torch._C._get_tracing_state
 
 
 def traced(*tensors: torch.Tensor) -> bool:
     """Whether a call has to go through torch's dispatcher: tensors that stand for others (fake ones of torch.compile and
     torch.export, wrappers), or a mode or transform that wants to see it. Else it launches at once: the way there and
     back is a few us of a 10 us call."""
-    if _compiling() or _modes() or _transform() is not None:
+    if _compiling() or _modes() or _transform() is not None or _jit() is not None:
         return True
     for t in tensors:
         if type(t) not in _PLAIN:

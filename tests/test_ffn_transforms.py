@@ -180,3 +180,31 @@ def test_traces_with_real_tensors_and_modes_see_the_operators():
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     o = torch.ops.cernels_b200
     assert o.gated_ffn_train.default in seen and o.gated_ffn_backward.default in seen
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+def test_jit_traces_record_the_operators():
+    """A trace made from one set of inputs computes with those of later calls."""
+    with torch.no_grad():
+        for name, f, args in calls("cuda"):
+            traced = torch.jit.trace(f, [a.clone() for a in args], check_trace=False)
+            other = [a * 0.5 for a in args]
+            assert torch.equal(traced(*other), f(*other)) and not torch.equal(f(*other), f(*args))
+
+
+@gpu
+def test_plain_subclasses_of_tensors_are_taken():
+    class Named(torch.Tensor):
+        pass
+
+    for name, f, args in calls("cuda"):
+        with torch.no_grad():
+            y = f(*(a.as_subclass(Named) for a in args))
+            assert isinstance(y, Named) and torch.equal(y.as_subclass(torch.Tensor), f(*args))
+    f, args = calls("cuda")[0][1:]
+    t, n = ([a.clone().requires_grad_() for a in args] for _ in range(2))
+    dy = torch.randn_like(args[0])
+    got = torch.autograd.grad(f(*(a.as_subclass(Named) for a in n)), n, dy.as_subclass(Named))
+    for g, w in zip(got, torch.autograd.grad(f(*t), t, dy)):
+        assert torch.equal(g.as_subclass(torch.Tensor), w)
