@@ -498,7 +498,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
   };
   auto store_x = [&](const Item& it, int mark, int first_chunk, const uint4 (&v)[kBatch]) {
     if constexpr (kFmt != 0) {
-      uint32_t large[kBatch / 4] = {0x04040404u, 0x04040404u};  // a byte for each chunk, 64 in all where there is none
+      // counts of large values, a byte for each block of two chunks, less the 64 that stand for a chunk which is not there
+      uint32_t large[kBatch / 2] = {};
       uint32_t special = 0;
 #pragma unroll
       for (int b = 0; b < kBatch; ++b) {
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
         const uint4 split_x = make_uint4(bytes(0x51, 0, 128), bytes(0x51, 1, 128), bytes(0x40, 0, 0), bytes(0x40, 1, 0));
         // values of 128 units or more, by their high byte; past the row's end half of the places count
         const uint32_t found = static_cast<int>(k8) * 8 < a.k ? __popc(nonzero_bytes(split_x.x) | nonzero_bytes(split_x.y) >> 1) : 4;
-        large[b / 4] += (found - 4) << 8 * (b % 4);
+        large[b / 2] += (found - 4) << (lane / 16 * 8 + b % 2 * 16);
         special = max(special, top);
         if (k8 % 16 == 0) units_of_x[c * blocks + k8 / 16] = __uint_as_float(static_cast<uint32_t>(unit_exp - 4) << 23);
         constexpr unsigned kPer = kFmt / 8;  // pieces per group
@@ -537,14 +538,13 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
         const unsigned at = k8 - in + (in % F::kWords) * 4 + in / F::kWords;
         *reinterpret_cast<uint4*>(xs + static_cast<size_t>(c) * x_bytes + at * 16) = split_x;
       }
-#pragma unroll
-      for (unsigned d = 8; d > 0; d /= 2)
-#pragma unroll
-        for (int j = 0; j < kBatch / 4; ++j) large[j] += __shfl_xor_sync(0xffffffffu, large[j], d);
       // a count under 64 in any block: bits 6 and 7 of its byte are clear
       uint32_t enough = 0x40404040u;
 #pragma unroll
-      for (int j = 0; j < kBatch / 4; ++j) enough &= large[j] | large[j] >> 1;
+      for (int j = 0; j < kBatch / 2; ++j) {
+        const uint32_t counts = __reduce_add_sync(0xffffffffu, large[j]) + 0x40404040u;
+        enough &= counts | counts >> 1;
+      }
       if (__any_sync(0xffffffffu, enough != 0x40404040u || special >= 0x7f800000u)) mark_mixed(it, mark, first_chunk);
     }
   };
@@ -641,9 +641,10 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     }
   };
   point_scales();
-  // The products of the unit's mixed blocks in this warp's steps, with codes, scales and x from global memory (L2 has
-  // them). The sums of integers left these blocks' columns out: their units are 0.
-  auto add_mixed = [&] {
+  // Adds the products of the unit's mixed blocks in this warp's steps to its sums `to` (in shared memory: registers for it
+  // would cost the loop of ordinary x), with codes, scales and x from global memory (L2 has them). The sums of integers
+  // left these blocks' columns out: their units are 0.
+  auto add_mixed = [&](float* to) {
     if constexpr (kFmt != 0) {
       const int base = (unit * tiles_at_once + rt) * kOut;
       const size_t e = routed ? item.expert : 0;
@@ -708,8 +709,8 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               if (kPacked ? j == 0 && mixed >> q & 1 : mixed >> (n * 8 + 2 * q + j) & 1) {
-                acc[n][j] = fmaf(scale_a[s], sum[j], acc[n][j]);
-                acc[n][j + 2] = fmaf(scale_b[s], sum[j + 2], acc[n][j + 2]);
+                to[n * 128 + j * 16] = fmaf(scale_a[s], sum[j], to[n * 128 + j * 16]);
+                to[n * 128 + j * 16 + 8] = fmaf(scale_b[s], sum[j + 2], to[n * 128 + j * 16 + 8]);
               }
             }
           }
@@ -836,7 +837,6 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
     if (++i == per_warp) {
       // ---- end of the unit: add the sums of each tile's warps (in warp order) and write
       i = 0;
-      if (any_mixed) add_mixed();
       float* mine = part + ((buffer * kWarps + warp) * kCols + (kPacked ? q : 2 * q)) * 16 + g;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -849,6 +849,7 @@ __global__ void __launch_bounds__(32 * kWarps, kWarps == 8 ? kCtas : 1) skinny_k
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[n][j] = 0.f;
       }
+      if (any_mixed) add_mixed(mine);
       __syncthreads();
       const float* all = part + buffer * kWarps * kCols * 16;
       // the half of the warps that adds first alternates, as there may be work for one half only
