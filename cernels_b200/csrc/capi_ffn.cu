@@ -54,10 +54,12 @@ int balanced_columns(int tokens, int k, int group) {
 
 // A few tokens: the weights' bytes bound the work, and the kernel that streams them (once per 16 tokens, or as
 // many as shared memory holds) beats the tile kernel, whose time is a full tile's for any number. By how much
-// more than once it may read them depends on whether L2 keeps them. us, streamed / tiled, at that many reads:
-//   50 MB (2880 x 2880)     3.0: 24.5 / 30.3   4.0: 36.0 / 30.3
-//   100 MB (8192 x 2048)    2.7: 35.4 / 48.0   3.3: 48.0 / 45.3     (4096 x 4096)  2.0: 39.2 / 38.3   3.0: 47.9 / 38.8
-//   302 MB (6144 x 8192)    1.0: 59.0 / 84.5   2.0: 80.2 / 72.0     402 MB (4096 x 16384)  1.7: 92.3 / 129.4
+// more than once it may read them depends on whether L2 keeps them. us, streamed / tiled, at T tokens and that many reads:
+//   50 MB (H = F = 2880)           T = 48, 3.0: 23.4 / 29.0    T = 64, 4.0: 35.0 / 29.0
+//   100 MB (H = 8192, F = 2048)    T = 30, 2.7: 44.7 / 48.5    T = 32, 3.3: 47.3 / 45.3
+//   100 MB (H = F = 4096)          T = 32, 2.0: 39.3 / 38.4    T = 48, 3.0: 54.8 / 38.7
+//   302 MB (H = 6144, F = 8192)    T = 10, 1.0: 62.0 / 82.8    T = 20, 2.0: 95.8 / 71.6
+//   402 MB (H = 4096, F = 16384)   T = 15, 1.7: 123.4 / 121.0
 bool few(const cernels_ffn_shape* s) {
   if (s->tokens > 4 * kSkinnyMaxColumns) return false;
   const int gate_up = passes_of(s->tokens, s->hidden, 0), down = passes_of(s->tokens, s->intermediate, 0);

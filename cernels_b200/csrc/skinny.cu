@@ -9,8 +9,8 @@
 // neighbouring warps read neighbouring bytes, and their sums are added in shared memory in warp order. A
 // CTA walks through a contiguous range of tiles with its x rows in shared memory and, per warp, the
 // weights of the next kDepth steps on their way into a ring of its own (cp.async, across tile borders): up to
-// 96 KB of weights in flight per SM. bf16 weights reach 5.5 of the measured 6.5 TB/s (one row of x, 201 MB in
-// 36.6 us). The same ring in registers gave 2.7 TB/s, and a third as much with 4-bit weights: a warp has too
+// 96 KB of weights in flight per SM. bf16 weights reach 5.3 of the measured 6.5 TB/s (one row of x, 201 MB in
+// 37.7 us). The same ring in registers gave 2.7 TB/s, and a third as much with 4-bit weights: a warp has too
 // few load counters to wait for one step and not for those behind it.
 //
 // mma.sync does the products: rows of W are the A operand, x columns the B operand. The order of k
@@ -35,8 +35,9 @@
 // The sums of 16 (q - 8) hi and 16 (q - 8) lo over a
 // group are exact integers of at most 128 * 128 * 128 < 2^22, and they start at the integer whose bits are the
 // float 1.5 * 2^23, so that their own bits are that float plus the sum. From there on it is 32-bit floating
-// arithmetic: scales are never rounded and multiply each group's sum. What bounds it now is instructions, 180 for 16 x 128 weights in groups of 32: experts
-// at 8 tokens take 87 us, without the copies 80, without the products 68, against 45 for their bytes.
+// arithmetic: scales are never rounded and multiply each group's sum. What bounds it now
+// is instructions, 180 for 16 x 128 weights in groups of 32: experts at 8 tokens take 86 us against 45 for their bytes (an
+// earlier state, at 87, took 80 without the copies and 68 without the products).
 #include "ffn_internal.h"
 
 #include <cmath>

@@ -84,8 +84,8 @@ def _linear_w4(x, qweight, scales):
 
 def linear_w4(x: torch.Tensor, qweight: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     """``x @ W.T`` for 4-bit W: x [T, K] bf16 (rows may lie apart), qweight [N, K / 2] uint8, scales
-    [N, K / G] bf16. Made for up to 16 rows, where the weights' bytes bound it; more rows work, and
-    read the weights once per 16."""
+    [N, K / G] bf16. Made for a few rows, where the weights' bytes bound it: they are read once for as many rows as
+    shared memory holds, at most 16 (16 up to K = 4864, 9 at 8192, 2 at 32768). More rows work."""
     if traced(x, qweight, scales):
         return _ops.linear_w4(x, qweight, scales)
     _check_no_grad(x, scales)

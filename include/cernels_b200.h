@@ -292,13 +292,15 @@ int cernels_gated_ffn_backward(const cernels_ffn_shape* shape, const void* x, in
  * aligned, a linear layer's scales 4-byte. */
 
 /* out[t, n] = sum_k x[t, k] W[n, k]: x [T, K] bf16 (row stride x_stride, a multiple of 8), out
- * [T, N] bf16. Bound by the weights' bytes up to 16 rows; more rows read them once per 16. */
+ * [T, N] bf16. The weights are read once for as many rows of x as shared memory holds, at most 16: 16 up to
+ * K = 4864, 12 at 6144, 9 at 8192, 5 at 16384, 2 at 32768. */
 int cernels_linear_w4(int32_t tokens, int32_t out_features, int32_t in_features, int32_t group, const void* x,
                       int64_t x_stride, const void* qweight, const void* scales, void* out, void* stream);
 
 /* cernels_moe_experts_decode with 4-bit experts (LINEAR layout): gate_up_q [E, 2F, H / 2], gate_up_scales
  * [E, 2F, H / group], down_q [E, H, F / 2], down_scales [E, H, F / group]; H and F multiples of group;
- * T * topk <= 1024. Each touched expert is read once per 8 tokens that chose it; ids outside [0, E) are
+ * T * topk <= 1024. A touched expert is read once for each 4 pairs that chose it, for each 8 where
+ * T * topk > 4 E (for fewer where H or F is too long for so many rows in shared memory); ids outside [0, E) are
  * skipped (a token with no expert gets zeros); deterministic. */
 int cernels_moe_w4_workspace_bytes(const cernels_moe_shape* shape, int32_t group, size_t* bytes);
 int cernels_moe_experts_decode_w4(const cernels_moe_shape* shape, int32_t group, const void* x, const void* gate_up_q,

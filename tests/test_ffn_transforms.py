@@ -208,3 +208,20 @@ def test_plain_subclasses_of_tensors_are_taken():
     got = torch.autograd.grad(f(*(a.as_subclass(Named) for a in n)), n, dy.as_subclass(Named))
     for g, w in zip(got, torch.autograd.grad(f(*t), t, dy)):
         assert torch.equal(g.as_subclass(torch.Tensor), w)
+
+
+@gpu
+def test_exported_programs_hold_the_operators():
+    class Call(torch.nn.Module):
+        def __init__(self, f):
+            super().__init__()
+            self.f = f
+
+        def forward(self, *args):
+            return self.f(*args)
+
+    for name, f, args in calls("cuda"):
+        with torch.no_grad():
+            program = torch.export.export(Call(f), tuple(args)).module()
+            other = [a * 0.5 for a in args]
+            assert torch.equal(program(*other), f(*other))
